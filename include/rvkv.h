@@ -515,6 +515,133 @@ int rvkv_sched_set_tokens(rvkv_sched *s, int64_t id, const int32_t *tokens,
                           uint32_t n);
 uint32_t rvkv_sched_refcount(const rvkv_sched *s, uint32_t block);
 
+/* ---- rotation by position, fused with the append ----------------
+ * Everything between the QKV projection and attention for models that
+ * rvkv_attn_prep does not cover: angles from the tokens' positions, the half
+ * or the interleaved pair layout, a rotation of the first rot_dim dims only,
+ * frequencies scaled for long contexts. The reference applies
+ * RotaryEmbedding's rotate-half form only (src/model.rs:224-250, 600-639).
+ * Row i, head h: optional x / sqrt(mean(x^2) + eps) * norm weight (q_norm,
+ * k_norm: f32 [head_dim] or NULL; v never), then for p < rot_dim / 2
+ *   angle = positions[i] * inv_freq[p],  c, s = attn_factor * cos, sin
+ *   (a, b) -> (a c - b s, a s + b c)
+ * over dims (p, p + rot_dim / 2), or (2p, 2p + 1) with interleaved 1; dims
+ * from rot_dim on stay. Evaluated in f64, rounded once. rot_dim 0: no
+ * rotation (positions and inv_freq may be NULL).
+ * q [rows, n_heads, head_dim], k and v [rows, n_kv_heads, head_dim] of dtype
+ * (F16 or F32), rows q_stride, k_stride, v_stride elements apart, heads of a
+ * row one behind the other (so slices of a fused QKV buffer are taken in
+ * place). The rotated q goes to q_out [rows, n_heads, head_dim] of dtype,
+ * which must not overlap the inputs; n_heads 0: no q (q and q_out may be
+ * NULL). k and v go to (slot_block[i], slot_off[i]) of `layer`; slots must be
+ * distinct within a call; a row whose slot is out of range still gives its
+ * q_out. positions, inv_freq (f32 [rot_dim / 2]), slots: device. head_dim <=
+ * 256, rot_dim even and <= head_dim, any strides and element alignment (16-byte
+ * aligned rows of head_dim 32, 64, 128 or 256 run the wide kernel). */
+int rvkv_rope_append(rvkv_pool *pool, uint32_t layer, const void *q,
+                     uint64_t q_stride, const void *k, uint64_t k_stride,
+                     const void *v, uint64_t v_stride, rvkv_dtype dtype,
+                     uint32_t rows, uint32_t n_heads, const float *q_norm,
+                     const float *k_norm, float eps, const uint32_t *positions,
+                     const float *inv_freq, uint32_t rot_dim,
+                     uint32_t interleaved, float attn_factor,
+                     const uint32_t *slot_block, const uint32_t *slot_off,
+                     void *q_out);
+
+/* ---- 8-bit paged cache --------------------------------------------
+ * A pool of its own kind (no counterpart in the reference): int8 codes with an
+ * f32 scale for every (token, KV head) of K and of V, head_dim + 4 bytes a
+ * row instead of 2 head_dim. A row x (K after its rotation) is stored as
+ *   scale = f32(max |x| / 127),  code = round(x / scale), ties to even,
+ * and stands for code * scale; a row with a value that is not finite is
+ * stored as NaN. The scale is a row's own, so a row's cells depend on nothing
+ * else that was written, and no append rewrites earlier rows.
+ * One block of one layer's K or V is a record of
+ *   ceil(n_kv * block_size * (head_dim + 4) / 256) * 256 bytes:
+ *   int8 codes, per KV head [block_size][head_dim] (K) or
+ *   [head_dim][block_size] (V), then f32 scales [n_kv][block_size];
+ * records [n_layers][K, V][num_blocks].
+ * head_dim: a multiple of 16, at most 256. block_size: a multiple of 16.
+ * Conventions as for rvkv_pool; besides, the calling thread's current device
+ * has to be the one the pool was created on (RVKV_EINVAL otherwise). */
+typedef struct rvkv_q8_pool rvkv_q8_pool;
+
+/* Bytes of such a pool's records; 0 for a shape that is refused. */
+size_t rvkv_q8_pool_bytes(uint32_t n_layers, uint32_t num_blocks,
+                          uint32_t block_size, uint32_t n_kv_heads,
+                          uint32_t head_dim);
+/* memory: device memory of at least rvkv_q8_pool_bytes(...) bytes, 256-byte
+ * aligned, that outlives the pool and is used as it is (a cache can be kept
+ * or shared that way); NULL: the pool allocates its own, zeroed. */
+int rvkv_q8_pool_create(uint32_t n_layers, uint32_t num_blocks,
+                        uint32_t block_size, uint32_t n_kv_heads,
+                        uint32_t head_dim, void *memory, size_t memory_bytes,
+                        rvkv_stream stream, rvkv_q8_pool **out);
+void rvkv_q8_pool_destroy(rvkv_q8_pool *pool);
+int rvkv_q8_pool_set_stream(rvkv_q8_pool *pool, rvkv_stream stream);
+
+/* rvkv_rope_append into an 8-bit pool. With n_heads 0 and rot_dim 0 it is the
+ * plain append (rvkv_append). */
+int rvkv_q8_rope_append(rvkv_q8_pool *pool, uint32_t layer, const void *q,
+                        uint64_t q_stride, const void *k, uint64_t k_stride,
+                        const void *v, uint64_t v_stride, rvkv_dtype dtype,
+                        uint32_t rows, uint32_t n_heads, const float *q_norm,
+                        const float *k_norm, float eps,
+                        const uint32_t *positions, const float *inv_freq,
+                        uint32_t rot_dim, uint32_t interleaved,
+                        float attn_factor, const uint32_t *slot_block,
+                        const uint32_t *slot_off, void *q_out);
+
+/* rvkv_gather of the cells' values into F32 or F16 (rounded). */
+int rvkv_q8_gather(const rvkv_q8_pool *pool, uint32_t layer,
+                   const uint32_t *block_idx, uint32_t batch,
+                   uint32_t max_blocks, uint32_t ctx_len, void *out_k,
+                   void *out_v, rvkv_dtype out_dtype);
+
+/* rvkv_copy_blocks: codes and scales, every layer, K and V. */
+int rvkv_q8_copy_blocks(rvkv_q8_pool *pool, const uint32_t *src,
+                        const uint32_t *dst, uint32_t n);
+
+/* rvkv_paged_decode over an 8-bit pool: q and out of dtype F16 or F32
+ * (either is computed to f32 accuracy, F16 rounded once at the end). Same
+ * rules for tables, ctx_lens, max_ctx_len, scale, window, empty contexts and
+ * workspace; besides, keys in a block whose table entry is >= num_blocks are
+ * left out (probability 0; the f16 pool's decode reads them as zeros).
+ * Contexts up to 2^32 - 256 tokens. Ragged batches need no plan: contexts are
+ * cut into partitions, and those behind a sequence's end cost nothing. */
+size_t rvkv_q8_decode_workspace_bytes(const rvkv_q8_pool *pool, uint32_t batch,
+                                      uint32_t n_heads, uint32_t max_ctx_len,
+                                      int32_t window);
+int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
+                         const void *q, rvkv_dtype dtype,
+                         const uint32_t *block_tables,
+                         const uint32_t *ctx_lens, uint32_t batch,
+                         uint32_t max_blocks, uint32_t n_heads,
+                         uint32_t max_ctx_len, float scale, int32_t window,
+                         void *out, void *ws, size_t ws_bytes);
+
+/* Attention of packed prompts, or chunks of prompts, of different lengths
+ * (rvkv_paged_prefill takes one length for all, src/model.rs:346-415): rows
+ * row_start[b] .. row_start[b + 1] - 1 of q and out belong to sequence b
+ * (row_start: device u32 [batch + 1], not decreasing). Row i of sequence b is
+ * at position pos_offset[b] + i and sees key j iff j < read_num_tokens[b],
+ * j <= its position and, with window > 0, j + window > its position; keys in
+ * a block whose table entry is >= num_blocks are left out. A row that sees no
+ * key gets zeros. Rows before row_start[0] and from row_start[batch] on are
+ * left as they were; total_rows is the number of rows that q and out hold
+ * (larger entries of row_start count as total_rows). q, out: [total_rows,
+ * n_heads, head_dim] of dtype, 16-byte aligned; F16 rounds the softmax
+ * weights once to f16, F32 is computed to f32 accuracy at about twice the
+ * matrix work. Contexts up to 2^32 - 256 tokens. */
+int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
+                           const void *q, rvkv_dtype dtype,
+                           const uint32_t *row_start, uint32_t total_rows,
+                           const uint32_t *block_tables,
+                           const uint32_t *pos_offset,
+                           const uint32_t *read_num_tokens, uint32_t batch,
+                           uint32_t max_blocks, uint32_t n_heads, float scale,
+                           int32_t window, void *out);
+
 #ifdef __cplusplus
 }
 #endif

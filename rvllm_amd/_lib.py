@@ -76,6 +76,24 @@ SIGNATURES = {
     "rvkv_bm_refcount": (_u32, [_P, _u32]),
     "rvkv_bm_table": (_int, [_P, _i64, _pu32, _u32]),
     "rvkv_argmax": (_int, [_P, _u32, _u32, _P, _P]),
+    "rvkv_rope_append": (_int, [_P, _u32, _P, _u64, _P, _u64, _P, _u64, _int,
+                                _u32, _u32, _P, _P, _f32, _P, _P, _u32, _u32,
+                                _f32, _P, _P, _P]),
+    "rvkv_q8_pool_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32]),
+    "rvkv_q8_pool_create": (_int, [_u32, _u32, _u32, _u32, _u32, _P, _sz, _P,
+                                   ctypes.POINTER(_P)]),
+    "rvkv_q8_pool_destroy": (None, [_P]),
+    "rvkv_q8_pool_set_stream": (_int, [_P, _P]),
+    "rvkv_q8_rope_append": (_int, [_P, _u32, _P, _u64, _P, _u64, _P, _u64,
+                                   _int, _u32, _u32, _P, _P, _f32, _P, _P,
+                                   _u32, _u32, _f32, _P, _P, _P]),
+    "rvkv_q8_gather": (_int, [_P, _u32, _P, _u32, _u32, _u32, _P, _P, _int]),
+    "rvkv_q8_copy_blocks": (_int, [_P, _P, _P, _u32]),
+    "rvkv_q8_decode_workspace_bytes": (_sz, [_P, _u32, _u32, _u32, _i32]),
+    "rvkv_q8_paged_decode": (_int, [_P, _u32, _P, _int, _P, _P, _u32, _u32,
+                                    _u32, _u32, _f32, _i32, _P, _P, _sz]),
+    "rvkv_q8_packed_prefill": (_int, [_P, _u32, _P, _int, _P, _u32, _P, _P, _P,
+                                      _u32, _u32, _u32, _f32, _i32, _P]),
     "rvkv_sched_last_error": (ctypes.c_char_p, []),
     "rvkv_sched_create": (_P, [_u32, _u32]),
     "rvkv_sched_destroy": (None, [_P]),

@@ -21,6 +21,9 @@ SOURCES = [
     os.path.join(HERE, "csrc", "prefill.hip"),
     os.path.join(HERE, "csrc", "argmax.hip"),
     os.path.join(HERE, "csrc", "generic.hip"),
+    os.path.join(HERE, "csrc", "rope_append.hip"),
+    os.path.join(HERE, "csrc", "q8.hip"),
+    os.path.join(HERE, "csrc", "q8_prefill.hip"),
     os.path.join(HERE, "csrc", "block_manager.cpp"),
     os.path.join(HERE, "csrc", "scheduler.cpp"),
 ]

@@ -1,0 +1,742 @@
+// q8.hip - the 8-bit paged cache's pool, its block copy and gather, and decode
+// attention over it.
+#include <new>
+
+#include "q8.h"
+
+using rvkv_detail::fail;
+using rvkv_detail::hip_fail;
+
+namespace rvkv_detail {
+int q8_device(const char *op, int device) {
+  int cur = -1;
+  const hipError_t e = hipGetDevice(&cur);
+  if (e != hipSuccess) return hip_fail(op, e);
+  if (cur != device)
+    return fail(RVKV_EINVAL, op, "the current device is not the pool's");
+  return RVKV_OK;
+}
+}  // namespace rvkv_detail
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Bytes of the records of a pool; 0 when the shape is refused (reason set).
+size_t q8_bytes(const char *op, uint32_t n_layers, uint32_t num_blocks,
+                uint32_t block_size, uint32_t n_kv, uint32_t hd, size_t *rec) {
+  if (n_layers == 0 || num_blocks == 0 || block_size == 0 || n_kv == 0 ||
+      hd == 0) {
+    fail(RVKV_EINVAL, op,
+         "n_layers/num_blocks/block_size/n_kv_heads/head_dim must be positive");
+    return 0;
+  }
+  if (hd % 16 || hd > 256) {
+    fail(RVKV_EUNSUPPORTED, op,
+         "head_dim must be a multiple of 16 and at most 256");
+    return 0;
+  }
+  if (block_size % 16 || block_size > 4096 || n_kv > 4096) {
+    fail(RVKV_EUNSUPPORTED, op,
+         "block_size must be a multiple of 16; block_size and n_kv_heads at "
+         "most 4096");
+    return 0;
+  }
+  *rec = ((size_t)n_kv * block_size * (hd + 4) + 255) & ~(size_t)255;
+  const unsigned __int128 all =
+      (unsigned __int128)*rec * num_blocks * 2 * n_layers;
+  if (all >> 48) {
+    fail(RVKV_EINVAL, op, "the pool is too large");
+    return 0;
+  }
+  return (size_t)all;
+}
+
+// ---------------------------------------------------------------------------
+// Gather: the cells' values, [batch, n_kv, ctx_len, hd]. One thread 16 dims of
+// a row; a block id out of range reads zeros.
+// ---------------------------------------------------------------------------
+template <typename Out>
+__global__ void __launch_bounds__(256)
+    q8_gather_kernel(const unsigned char *kc, const unsigned char *vc,
+                     size_t rec, const uint32_t *tables, Out *out_k, Out *out_v,
+                     uint64_t n, uint32_t max_blocks, uint32_t ctx_len,
+                     uint32_t n_kv, uint32_t hd, uint32_t bs,
+                     uint32_t num_blocks) {
+  const uint32_t chunks = hd / 16;
+  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const uint64_t row = i / chunks;
+  const uint32_t d0 = (uint32_t)(i - row * chunks) * 16;
+  const uint32_t tok = (uint32_t)(row % ctx_len);
+  const uint64_t bh = row / ctx_len;
+  const uint32_t head = (uint32_t)(bh % n_kv);
+  const uint32_t blk = tables[bh / n_kv * max_blocks + tok / bs];
+  const uint32_t off = tok % bs;
+  const bool is_v = blockIdx.y;
+  Out *out = (is_v ? out_v : out_k) + row * hd + d0;
+  if (blk >= num_blocks) {
+    for (int e = 0; e < 16; ++e) out[e] = (Out)0.f;
+    return;
+  }
+  const unsigned char *block = (is_v ? vc : kc) + blk * rec;
+  const float scale = *reinterpret_cast<const float *>(
+      block + (size_t)n_kv * bs * hd + ((size_t)head * bs + off) * 4);
+  const signed char *tile =
+      reinterpret_cast<const signed char *>(block) + (size_t)head * bs * hd;
+  for (int e = 0; e < 16; ++e)
+    out[e] = (Out)((float)(is_v ? tile[(size_t)(d0 + e) * bs + off]
+                                : tile[(size_t)off * hd + d0 + e]) *
+                   scale);
+}
+
+__global__ void __launch_bounds__(256)
+    q8_copy_kernel(unsigned char *base, size_t tensor_bytes, size_t rec,
+                   const uint32_t *src, const uint32_t *dst,
+                   uint32_t num_blocks) {
+  const uint32_t s = src[blockIdx.y], d = dst[blockIdx.y];
+  if (s >= num_blocks || d >= num_blocks) return;
+  unsigned char *t = base + (size_t)blockIdx.z * tensor_bytes;
+  const uint4 *from = reinterpret_cast<const uint4 *>(t + s * rec);
+  uint4 *to = reinterpret_cast<uint4 *>(t + d * rec);
+  for (size_t w = (size_t)blockIdx.x * 256 + threadIdx.x; w < rec / 16;
+       w += (size_t)gridDim.x * 256)
+    to[w] = from[w];
+}
+
+// ---------------------------------------------------------------------------
+// Decode attention.
+//
+//   s_j = scale ks_j (q . kcode_j),   out = sum_j p_j vs_j vcode_j / sum_j p_j,
+//   p_j = exp(s_j - max s), all keys j < ctx (and >= ctx - window).
+//
+// Both products run on v_mfma_f32_16x16x32_f16 with the keys, or the dims, as
+// the 16 rows and the heads of a KV group as the 16 columns: codes are exact
+// in f16, and the columns that a group of up to 8 heads leaves free carry the
+// f16 remainders of q and of the weights (column c the upper part of head c,
+// column c + 8 the lower), so q and the weights keep 21 bits or more and the
+// result is an f32 one at no extra product. Larger groups take n_sub
+// workgroups of up to 8 heads.
+//
+// A wave takes 64 keys at a time and the workgroup's four waves take turns.
+// Row 4g + i of S tile t is key 16g + 4t + i, so lane group g of the result
+// holds keys 16g .. 16g+15: the order in which the V' P product takes its
+// weights from the same registers, and 16 keys of one dim are 16 bytes of a
+// V record. No operand passes through LDS.
+// ---------------------------------------------------------------------------
+struct DecodeArgs {
+  const void *q;
+  void *out;
+  const unsigned char *kc, *vc;
+  const uint32_t *tables, *ctx_lens;
+  float *ws_acc, *ws_ml;
+  size_t rec;
+  uint32_t n_heads, n_kv, group, n_sub, hd, bs, max_blocks, num_blocks;
+  uint32_t ctx_cap, part_tokens, n_parts;
+  float qscale;  // scale * log2(e)
+  uint32_t window;
+};
+
+// A sequence's visible keys [lo, ctx); its partitions start at base, lo
+// rounded down to whole records' granules of 16 keys.
+struct Range {
+  uint32_t ctx, lo, base;
+};
+__device__ __forceinline__ Range visible(const DecodeArgs &a, uint32_t b) {
+  Range r;
+  r.ctx = a.ctx_lens[b];
+  if (r.ctx > a.ctx_cap) r.ctx = a.ctx_cap;
+  r.lo = a.window && r.ctx > a.window ? r.ctx - a.window : 0;
+  r.base = r.lo & ~15u;
+  return r;
+}
+
+__device__ __forceinline__ float ror8(float x) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x128,
+                                                  0xf, 0xf, true));
+}
+__device__ __forceinline__ float max_groups(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ half2v pk(float a, float b) {
+  return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) q8_decode_kernel(DecodeArgs a) {
+  constexpr int NK = HD / 64, NV = HD / 16;
+  constexpr float kNone = -__builtin_inff();
+  __shared__ float sh_acc[4][8][HD];
+  __shared__ float sh_m[4][8], sh_l[4][8];
+  const uint32_t part = blockIdx.x, b = blockIdx.z;
+  const uint32_t kvh = blockIdx.y / a.n_sub, sub = blockIdx.y % a.n_sub;
+  const Range rg = visible(a, b);
+  const uint64_t start64 = (uint64_t)rg.base + (uint64_t)part * a.part_tokens;
+  if (a.n_parts > 1 && start64 >= rg.ctx) return;
+  const uint32_t start = (uint32_t)start64;
+  const uint32_t end = rg.ctx - start < a.part_tokens ? rg.ctx
+                                                      : start + a.part_tokens;
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t col = lane & 15, g = lane >> 4;
+  const uint32_t h_in = sub * 8 + (col & 7);
+  const bool has_head = h_in < a.group;
+  const uint32_t head = kvh * a.group + (has_head ? h_in : 0);
+  const uint32_t hd = a.hd, bs = a.bs, bsg = bs / 16;
+
+  // q of this lane's column: element u * 8 + j of chunk c is dim
+  // 64 c + 16 g + 8 u + j. Brought just below 2^15 by a power of two: neither
+  // part leaves f16's range, the lower one not its normal numbers.
+  half8v qf[NK][2];
+  float qscale = a.qscale;
+  {
+    const T *q = (const T *)a.q + ((size_t)b * a.n_heads + head) * hd;
+    float x[NK][16];
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t d = 64 * c + 16 * g + e;
+        x[c][e] = has_head && d < hd ? (float)q[d] : 0.f;
+        top = fmaxf(top, fabsf(x[c][e]));
+      }
+    top = max_groups(top);
+    const uint32_t ex = scale_exponent(top);
+    const float down = __uint_as_float((269 - ex) << 23);
+    qscale *= __uint_as_float((ex - 15) << 23);
+    const float part_of = col >= 8 ? 1.f : 0.f;
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float y = x[c][e] * down;
+        qf[c][e >> 3][e & 7] =
+            (_Float16)__builtin_fmaf(-part_of, (float)(_Float16)y, y);
+      }
+  }
+
+  const uint32_t n_tiles = end > start ? (end - start + 63) / 64 : 0;
+  const uint32_t last_granule = rg.ctx ? (rg.ctx - 1) / 16 : 0;
+  const uint32_t *table = a.tables + (size_t)b * a.max_blocks;
+  // Block id and granule within the block of key granule gr (clamped to the
+  // sequence's last: keys behind it are masked).
+  struct Place {
+    uint32_t blk, in;
+  };
+  const auto place = [&](uint32_t tile, uint32_t gr) {
+    uint32_t x = (start + tile * 64) / 16 + gr;
+    x = x < last_granule ? x : last_granule;
+    Place p;
+    const uint32_t bi = bsg == 1 ? x : x / bsg;
+    p.in = x - bi * bsg;
+    p.blk = table[bi];
+    return p;
+  };
+  uint4 kr[4 * NK], vr[NV];
+  float ks[16], vs[16];
+  bool seen;  // this lane group's keys lie in a readable block
+  const uint32_t gk = col >> 2;
+  const auto load_k = [&](Place p) {
+    const uint32_t blk = p.blk < a.num_blocks ? p.blk : 0;
+    const unsigned char *kp = a.kc + blk * a.rec + (size_t)kvh * bs * hd +
+                              (p.in * 16 + (col & 3)) * hd + g * 16;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+        kr[t * NK + c] = *reinterpret_cast<const uint4 *>(
+            kp + t * 4 * hd + (c * 64 + g * 16 < hd ? c * 64 : 0));
+  };
+  const auto load_scales = [&](Place p) {
+    seen = p.blk < a.num_blocks;
+    const uint32_t blk = seen ? p.blk : 0;
+    const size_t at = blk * a.rec + (size_t)a.n_kv * bs * hd +
+                      ((size_t)kvh * bs + p.in * 16) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<float4 *>(ks + 4 * i) =
+          *reinterpret_cast<const float4 *>(a.kc + at + 16 * i);
+      *reinterpret_cast<float4 *>(vs + 4 * i) =
+          *reinterpret_cast<const float4 *>(a.vc + at + 16 * i);
+    }
+  };
+  const auto load_v = [&](Place p) {
+    const uint32_t blk = p.blk < a.num_blocks ? p.blk : 0;
+    const unsigned char *vp = a.vc + blk * a.rec + (size_t)kvh * bs * hd +
+                              col * bs + p.in * 16;
+#pragma unroll
+    for (int d = 0; d < NV; ++d)
+      if ((uint32_t)d * 16 < hd)
+        vr[d] = *reinterpret_cast<const uint4 *>(vp + d * 16 * bs);
+  };
+
+  float m = kNone, l = 0.f;
+  float vnorm = kVnorm0;  // power of two above every vs
+  float4v acc[NV];
+#pragma unroll
+  for (int d = 0; d < NV; ++d) acc[d] = float4v{0.f, 0.f, 0.f, 0.f};
+  const float lower = col >= 8 ? 1.f : 0.f;
+
+  if (wave < n_tiles) {
+    Place pk0 = place(wave, gk), pv0 = place(wave, g);
+    Place pk1 = place(wave + 4, gk), pv1 = place(wave + 4, g);
+    load_k(pk0);
+    load_scales(pv0);
+    load_v(pv0);
+    for (uint32_t tile = wave; tile < n_tiles; tile += 4) {
+      const bool more = tile + 4 < n_tiles;
+      float s[16];
+      {
+        float4v st[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          st[t] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NK; ++c) {
+            const uint4 k = kr[t * NK + c];
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                codes_to_half8(k.x, k.y), qf[c][0], st[t], 0, 0, 0);
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                codes_to_half8(k.z, k.w), qf[c][1], st[t], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = st[j >> 2][j & 3];
+      }
+      if (more) load_k(pk1);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = (s[j] + ror8(s[j])) * (ks[j] * qscale);
+      const uint32_t key = start + tile * 64 + 16 * g;
+      if (start + tile * 64 < rg.lo || start + tile * 64 + 64 > end ||
+          !__all(seen)) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const bool ok = seen && key + j >= rg.lo && key + j < end;
+          s[j] = ok ? s[j] : kNone;
+          vs[j] = ok ? vs[j] : 0.f;
+        }
+      }
+      float top = s[0], vtop = vs[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) {
+        top = fmaxf(top, s[j]);
+        vtop = fmaxf(vtop, vs[j]);
+      }
+      const float m_new = fmaxf(m, max_groups(top));
+      vtop = max_groups(vtop);
+      const float mm = m_new == kNone ? 0.f : m_new;
+      float fix = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+      if (m == m_new) fix = 1.f;
+      m = m_new;
+      l *= fix;
+      if (vtop >= vnorm) {  // (uniform over the wave)
+        uint32_t e = (__float_as_uint(vtop) >> 23) + 1;
+        e = e > 253 ? 253 : e;
+        const float now = __uint_as_float(e << 23);
+        fix *= vnorm / now;
+        vnorm = now;
+      }
+      if (!__all(fix == 1.f)) {
+#pragma unroll
+        for (int d = 0; d < NV; ++d) acc[d] *= fix;
+      }
+      // (weights up to 2^15, as q)
+      const float vdown =
+          __uint_as_float((269u << 23) - __float_as_uint(vnorm));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float p = __builtin_amdgcn_exp2f(s[j] - mm);
+        l += p;
+        s[j] = p * (vs[j] * vdown);
+      }
+      if (more) load_scales(pv1);
+      half8v pf[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float w0 = s[8 * u + j], w1 = s[8 * u + j + 1];
+          const half2v up = pk(w0, w1);
+          const half2v x = pk(__builtin_fmaf(-lower, (float)up[0], w0),
+                              __builtin_fmaf(-lower, (float)up[1], w1));
+          pf[u][j] = x[0];
+          pf[u][j + 1] = x[1];
+        }
+#pragma unroll
+      for (int d = 0; d < NV; ++d) {
+        if ((uint32_t)d * 16 < hd) {
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              codes_to_half8(vr[d].x, vr[d].y), pf[0], acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              codes_to_half8(vr[d].z, vr[d].w), pf[1], acc[d], 0, 0, 0);
+        }
+      }
+      if (more) {
+        load_v(pv1);
+        pk1 = place(tile + 8, gk);
+        pv1 = place(tile + 8, g);
+      }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+  }
+
+  // Merge the waves: a head's weights relative to the largest maximum.
+  if (lane < 8) {
+    sh_m[wave][lane] = m;
+    sh_l[wave][lane] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < NV; ++d) {
+    float4v o = acc[d];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (o[i] + ror8(o[i])) * (vnorm * 0x1p-15f);
+    if (col < 8)
+      *reinterpret_cast<float4v *>(&sh_acc[wave][col][d * 16 + 4 * g]) = o;
+  }
+  __syncthreads();
+  for (uint32_t x = threadIdx.x; x < 8 * HD; x += 256) {
+    const uint32_t h = x / HD, d = x % HD;
+    if (sub * 8 + h >= a.group || d >= hd) continue;
+    float top = sh_m[0][h];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, sh_m[w][h]);
+    float o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = sh_m[w][h] == kNone ? 0.f : __builtin_amdgcn_exp2f(sh_m[w][h] - top);
+      o += sh_acc[w][h][d] * f;
+      sum += sh_l[w][h] * f;
+    }
+    const size_t row = (size_t)b * a.n_heads + kvh * a.group + sub * 8 + h;
+    if (a.n_parts == 1) {
+      ((T *)a.out)[row * hd + d] = (T)(sum == 0.f ? 0.f : o / sum);
+    } else {
+      const size_t slot = row * a.n_parts + part;
+      a.ws_acc[slot * HD + d] = o;
+      if (d == 0) {
+        a.ws_ml[slot * 2] = top;
+        a.ws_ml[slot * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// Merges a head's partitions: 256 threads, 256 / HD partitions at a time.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) q8_reduce_kernel(DecodeArgs a) {
+  constexpr int W = 256 / HD;
+  constexpr float kNone = -__builtin_inff();
+  __shared__ float sh_o[256], sh_l[W];
+  const uint32_t h = blockIdx.x, b = blockIdx.y;
+  const Range rg = visible(a, b);
+  const uint32_t live =
+      rg.ctx > rg.base
+          ? (rg.ctx - rg.base + a.part_tokens - 1) / a.part_tokens : 0;
+  const size_t row = (size_t)b * a.n_heads + h;
+  const float *ml = a.ws_ml + row * a.n_parts * 2;
+  const float *acc = a.ws_acc + row * a.n_parts * HD;
+  const uint32_t d = threadIdx.x % HD, w = threadIdx.x / HD;
+  float top = kNone;
+  for (uint32_t p = 0; p < live; ++p) top = fmaxf(top, ml[2 * p]);
+  float o = 0.f, sum = 0.f;
+  for (uint32_t p = w; p < live; p += W) {
+    const float f = ml[2 * p] == kNone ? 0.f : __builtin_amdgcn_exp2f(ml[2 * p] - top);
+    sum += ml[2 * p + 1] * f;
+    if (d < a.hd) o += acc[(size_t)p * HD + d] * f;
+  }
+  sh_o[threadIdx.x] = o;
+  if (d == 0) sh_l[w] = sum;
+  __syncthreads();
+  if (w == 0 && d < a.hd) {
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      o += sh_o[i * HD + d];
+      sum += sh_l[i];
+    }
+    ((T *)a.out)[row * a.hd + d] = (T)(sum == 0.f ? 0.f : o / sum);
+  }
+}
+
+uint32_t hd_up(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+// Keys of a partition, a multiple of 256 (64 for each of the four waves).
+uint32_t partition_tokens(const rvkv_q8_pool *p, uint32_t batch,
+                          uint32_t n_heads, uint32_t keys) {
+  const uint32_t n_sub = (n_heads / p->n_kv + 7) / 8;
+  const uint64_t rows = (uint64_t)batch * p->n_kv * n_sub;
+  const uint64_t want = ((uint64_t)keys * rows + 1023) / 1024;
+  uint64_t t = (want + 255) / 256 * 256;
+  return (uint32_t)(t < 256 ? 256 : t > 1024 ? 1024 : t);
+}
+
+struct Layout {
+  uint32_t part_tokens, n_parts;
+  size_t ml_off, bytes;
+};
+// window 0: none. A window's first partition starts up to 15 keys before it.
+Layout layout(const rvkv_q8_pool *p, uint32_t batch, uint32_t n_heads,
+              uint32_t max_ctx, uint32_t window) {
+  Layout w{};
+  uint64_t keys = max_ctx ? max_ctx : 1;
+  if (window && (uint64_t)window + 15 < keys) keys = (uint64_t)window + 15;
+  w.part_tokens = partition_tokens(p, batch, n_heads, (uint32_t)keys);
+  w.n_parts = (uint32_t)((keys + w.part_tokens - 1) / w.part_tokens);
+  if (w.n_parts <= 1) return w;
+  const size_t slots = (size_t)batch * n_heads * w.n_parts;
+  w.ml_off = slots * hd_up(p->head_dim) * 4;
+  w.bytes = (w.ml_off + slots * 8 + 255) & ~(size_t)255;
+  return w;
+}
+
+template <typename T, int HD>
+int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
+                  hipStream_t st) {
+  hipLaunchKernelGGL((q8_decode_kernel<T, HD>),
+                     dim3(a.n_parts, a.n_kv * a.n_sub, batch), dim3(256), 0, st,
+                     a);
+  if (a.n_parts > 1)
+    hipLaunchKernelGGL((q8_reduce_kernel<T, HD>), dim3(a.n_heads, batch),
+                       dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
+}
+
+template <typename T>
+int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
+                  hipStream_t st) {
+  switch (hd_up(a.hd)) {
+    case 64: return launch_decode<T, 64>(op, a, batch, st);
+    case 128: return launch_decode<T, 128>(op, a, batch, st);
+    default: return launch_decode<T, 256>(op, a, batch, st);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rvkv_q8_pool_bytes(uint32_t n_layers, uint32_t num_blocks,
+                          uint32_t block_size, uint32_t n_kv_heads,
+                          uint32_t head_dim) {
+  size_t rec;
+  return q8_bytes("q8_pool_bytes", n_layers, num_blocks, block_size,
+                  n_kv_heads, head_dim, &rec);
+}
+
+int rvkv_q8_pool_create(uint32_t n_layers, uint32_t num_blocks,
+                        uint32_t block_size, uint32_t n_kv_heads,
+                        uint32_t head_dim, void *memory, size_t memory_bytes,
+                        rvkv_stream stream, rvkv_q8_pool **out) {
+  const char *op = "q8_pool_create";
+  if (!out) return fail(RVKV_EINVAL, op, "out is NULL");
+  *out = nullptr;
+  size_t rec = 0;
+  const size_t bytes = q8_bytes(op, n_layers, num_blocks, block_size,
+                                n_kv_heads, head_dim, &rec);
+  if (!bytes)
+    return head_dim % 16 || head_dim > 256 || block_size % 16 ||
+                   block_size > 4096 || n_kv_heads > 4096
+               ? RVKV_EUNSUPPORTED : RVKV_EINVAL;
+  if (memory && memory_bytes < bytes)
+    return fail(RVKV_EINVAL, op, "memory smaller than the required bytes");
+  if ((uintptr_t)memory % 256)
+    return fail(RVKV_EINVAL, op, "memory must be 256-byte aligned");
+  int device = -1;
+  hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    // (the caller's memory needs no device yet; every launch asks again)
+    if (!memory) return hip_fail(op, e);
+    device = -1;
+  }
+  rvkv_q8_pool *p = new (std::nothrow) rvkv_q8_pool();
+  if (!p) return fail(RVKV_ENOMEM, op, "out of host memory");
+  p->n_layers = n_layers;
+  p->num_blocks = num_blocks;
+  p->block_size = block_size;
+  p->n_kv = n_kv_heads;
+  p->head_dim = head_dim;
+  p->rec = rec;
+  p->tensor_bytes = rec * num_blocks;
+  p->stream = static_cast<hipStream_t>(stream);
+  p->device = device;
+  p->base = static_cast<unsigned char *>(memory);
+  if (!memory) {
+    e = hipMalloc(&p->base, bytes);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      delete p;
+      return fail(RVKV_ENOMEM, op, "hipMalloc of the pool failed");
+    }
+    p->owned = true;
+    e = hipMemsetAsync(p->base, 0, bytes, p->stream);
+    if (e != hipSuccess) {
+      (void)hipFree(p->base);
+      delete p;
+      return hip_fail(op, e);
+    }
+  }
+  *out = p;
+  return RVKV_OK;
+}
+
+void rvkv_q8_pool_destroy(rvkv_q8_pool *pool) {
+  if (!pool) return;
+  if (pool->owned) {
+    (void)hipStreamSynchronize(pool->stream);
+    (void)hipFree(pool->base);
+  }
+  delete pool;
+}
+
+int rvkv_q8_pool_set_stream(rvkv_q8_pool *pool, rvkv_stream stream) {
+  if (!pool) return fail(RVKV_EINVAL, "q8_pool_set_stream", "pool is NULL");
+  pool->stream = static_cast<hipStream_t>(stream);
+  return RVKV_OK;
+}
+
+int rvkv_q8_gather(const rvkv_q8_pool *pool, uint32_t layer,
+                   const uint32_t *block_idx, uint32_t batch,
+                   uint32_t max_blocks, uint32_t ctx_len, void *out_k,
+                   void *out_v, rvkv_dtype out_dtype) {
+  const char *op = "kv_gather";
+  if (!pool) return fail(RVKV_EINVAL, op, "pool is NULL");
+  if (layer >= pool->n_layers)
+    return fail(RVKV_EINVAL, op, "layer out of range");
+  if (batch == 0 || max_blocks == 0 || ctx_len == 0)
+    return fail(RVKV_EINVAL, op,
+                "batch/max_blocks/ctx_len/block_size/n_kv_heads/head_dim must "
+                "be positive");
+  if ((uint64_t)ctx_len > (uint64_t)max_blocks * pool->block_size)
+    return fail(RVKV_EINVAL, op,
+                "ctx_len must not exceed max_blocks * block_size");
+  if (!block_idx || !out_k || !out_v)
+    return fail(RVKV_EINVAL, op, "NULL block_idx/out_k/out_v");
+  if (out_dtype != RVKV_F16 && out_dtype != RVKV_F32)
+    return fail(RVKV_EINVAL, op, "out dtype must be F16 or F32");
+  const uint64_t n = (uint64_t)batch * pool->n_kv * ctx_len *
+                     (pool->head_dim / 16);
+  if ((n + 255) / 256 > 0x7fffffffull)
+    return fail(RVKV_EUNSUPPORTED, op, "too many rows for one launch");
+  const int rc = rvkv_detail::q8_device(op, pool->device);
+  if (rc) return rc;
+  const dim3 grid((uint32_t)((n + 255) / 256), 2);
+  if (out_dtype == RVKV_F16)
+    hipLaunchKernelGGL(q8_gather_kernel<_Float16>, grid, dim3(256), 0,
+                       pool->stream, pool->tensor(layer, 0),
+                       pool->tensor(layer, 1), pool->rec, block_idx,
+                       (_Float16 *)out_k, (_Float16 *)out_v, n, max_blocks,
+                       ctx_len, pool->n_kv, pool->head_dim, pool->block_size,
+                       pool->num_blocks);
+  else
+    hipLaunchKernelGGL(q8_gather_kernel<float>, grid, dim3(256), 0,
+                       pool->stream, pool->tensor(layer, 0),
+                       pool->tensor(layer, 1), pool->rec, block_idx,
+                       (float *)out_k, (float *)out_v, n, max_blocks, ctx_len,
+                       pool->n_kv, pool->head_dim, pool->block_size,
+                       pool->num_blocks);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
+}
+
+int rvkv_q8_copy_blocks(rvkv_q8_pool *pool, const uint32_t *src,
+                        const uint32_t *dst, uint32_t n) {
+  const char *op = "copy_blocks";
+  if (!pool) return fail(RVKV_EINVAL, op, "pool is NULL");
+  if (n == 0) return RVKV_OK;
+  if (!src || !dst) return fail(RVKV_EINVAL, op, "NULL src/dst");
+  if (n > 65535)
+    return fail(RVKV_EUNSUPPORTED, op, "at most 65535 pairs per call");
+  if (pool->n_layers > 32767)
+    return fail(RVKV_EUNSUPPORTED, op, "too many layers");
+  const int rc = rvkv_detail::q8_device(op, pool->device);
+  if (rc) return rc;
+  size_t gx = (pool->rec / 16 + 255) / 256;
+  if (gx > 64) gx = 64;
+  hipLaunchKernelGGL(q8_copy_kernel, dim3((uint32_t)gx, n, 2 * pool->n_layers),
+                     dim3(256), 0, pool->stream, pool->base,
+                     pool->tensor_bytes, pool->rec, src, dst,
+                     pool->num_blocks);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
+}
+
+size_t rvkv_q8_decode_workspace_bytes(const rvkv_q8_pool *pool, uint32_t batch,
+                                      uint32_t n_heads, uint32_t max_ctx_len,
+                                      int32_t window) {
+  if (!pool || batch == 0 || n_heads == 0 || n_heads % pool->n_kv) return 0;
+  return layout(pool, batch, n_heads, max_ctx_len,
+                window > 0 ? (uint32_t)window : 0).bytes;
+}
+
+int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
+                         const void *q, rvkv_dtype dtype,
+                         const uint32_t *block_tables,
+                         const uint32_t *ctx_lens, uint32_t batch,
+                         uint32_t max_blocks, uint32_t n_heads,
+                         uint32_t max_ctx_len, float scale, int32_t window,
+                         void *out, void *ws, size_t ws_bytes) {
+  const char *op = "paged_decode";
+  if (!pool) return fail(RVKV_EINVAL, op, "pool is NULL");
+  if (layer >= pool->n_layers)
+    return fail(RVKV_EINVAL, op, "layer out of range");
+  if (dtype != RVKV_F16 && dtype != RVKV_F32)
+    return fail(RVKV_EINVAL, op, "dtype must be F16 or F32");
+  if (batch == 0) return RVKV_OK;
+  if (batch > 65535) return fail(RVKV_EUNSUPPORTED, op, "batch too large");
+  if (max_blocks == 0)
+    return fail(RVKV_EINVAL, op, "max_blocks must be positive");
+  if (n_heads == 0 || n_heads % pool->n_kv != 0)
+    return fail(RVKV_EINVAL, op,
+                "n_heads must be a positive multiple of n_kv_heads");
+  if (!q || !block_tables || !ctx_lens || !out)
+    return fail(RVKV_EINVAL, op, "NULL q/block_tables/ctx_lens/out");
+  if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
+    return fail(RVKV_EINVAL, op, "q and out must be 16-byte aligned");
+  const uint32_t group = n_heads / pool->n_kv, n_sub = (group + 7) / 8;
+  if ((uint64_t)pool->n_kv * n_sub > 65535)
+    return fail(RVKV_EUNSUPPORTED, op, "head count too large");
+  const uint64_t cap = (uint64_t)max_blocks * pool->block_size;
+  if (max_ctx_len == 0) max_ctx_len = 1;
+  if (max_ctx_len > rvkv_detail::kMaxKeys) max_ctx_len = rvkv_detail::kMaxKeys;
+  const Layout w = layout(pool, batch, n_heads, max_ctx_len,
+                          window > 0 ? (uint32_t)window : 0);
+  if (w.bytes) {
+    if (!ws) return fail(RVKV_EINVAL, op, "workspace is NULL");
+    if (ws_bytes < w.bytes)
+      return fail(RVKV_EINVAL, op, "workspace smaller than the required bytes");
+    if ((uintptr_t)ws % 256)
+      return fail(RVKV_EINVAL, op, "workspace must be 256-byte aligned");
+  }
+  const int rc = rvkv_detail::q8_device(op, pool->device);
+  if (rc) return rc;
+  DecodeArgs a{};
+  a.q = q;
+  a.out = out;
+  a.kc = pool->tensor(layer, 0);
+  a.vc = pool->tensor(layer, 1);
+  a.tables = block_tables;
+  a.ctx_lens = ctx_lens;
+  a.ws_acc = static_cast<float *>(ws);
+  a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.ml_off);
+  a.rec = pool->rec;
+  a.n_heads = n_heads;
+  a.n_kv = pool->n_kv;
+  a.group = group;
+  a.n_sub = n_sub;
+  a.hd = pool->head_dim;
+  a.bs = pool->block_size;
+  a.max_blocks = max_blocks;
+  a.num_blocks = pool->num_blocks;
+  a.ctx_cap = (uint32_t)(cap < max_ctx_len ? cap : max_ctx_len);
+  a.part_tokens = w.part_tokens;
+  a.n_parts = w.n_parts;
+  a.qscale = scale * kLog2e;
+  a.window = window > 0 ? (uint32_t)window : 0;
+  return dtype == RVKV_F16 ? launch_decode<_Float16>(op, a, batch, pool->stream)
+                           : launch_decode<float>(op, a, batch, pool->stream);
+}
+
+}  // extern "C"

@@ -45,6 +45,60 @@ def _dev_u32(x, device) -> torch.Tensor:
     return torch.from_numpy(arr.copy()).to(device)
 
 
+def rope_append_call(fn, store, layer: int, q, k, v, positions, inv_freq,
+                     slot_block, slot_off, interleaved, attn_factor, q_norm,
+                     k_norm, eps, q_out):
+    """rvkv_rope_append / rvkv_q8_rope_append (fn) with what the C ABI cannot
+    see checked first. q None: no query heads; inv_freq None: no rotation."""
+    hd, kv = store.head_dim, store.n_kv_heads
+    op = "rope_append"
+    rows = int(k.shape[0])
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t is None and name == "q":
+            continue
+        _need(t.dim() == 3 and t.shape[0] == rows and t.shape[2] == hd and
+              (name == "q" or t.shape[1] == kv),
+              f"{op}: {name} must be [rows, heads, head_dim]")
+        _need(t.dtype == k.dtype and t.dtype in _DT,
+              f"{op}: q/k/v must all be float32 or float16")
+        # (the stride of a dimension of size 1 is of no account)
+        _need((hd == 1 or t.stride(2) == 1) and
+              (t.shape[1] == 1 or t.stride(1) == hd),
+              f"{op}: a row's heads must lie one behind the other")
+    n_heads = 0 if q is None else int(q.shape[1])
+    rot = 0 if inv_freq is None else 2 * int(inv_freq.numel())
+    ints = [slot_block, slot_off] + ([positions] if rot else [])
+    for t in ints:
+        _need(t.numel() == rows and t.dtype == torch.int32 and
+              t.is_contiguous(),
+              f"{op}: positions/block_ids/offsets must be contiguous int32, "
+              "one per row")
+    floats = [(inv_freq, None), (q_norm, hd), (k_norm, hd)]
+    for t, n in floats:
+        _need(t is None or (t.dtype == torch.float32 and t.is_contiguous() and
+                            (n is None or t.numel() == n)),
+              f"{op}: inv_freq and norm weights must be contiguous float32, "
+              "norm weights [head_dim]")
+    if q is not None and q_out is None:
+        q_out = torch.empty((rows, n_heads, hd), dtype=q.dtype,
+                            device=q.device)
+    _need(q is None or (q_out.shape == q.shape and q_out.dtype == q.dtype and
+                        q_out.is_contiguous()),
+          f"{op}: q_out must be contiguous and match q")
+    for t in [q, k, v, q_out, *ints, *(t for t, _ in floats)]:
+        _need(t is None or t.device == store.device,
+              f"{op}: every tensor must be on the storage's device")
+    # (one row's stride is of no account: 0 rows apart)
+    stride = [0 if t is None else (t.stride(0) if rows > 1 else
+                                   t.shape[1] * hd) for t in (q, k, v)]
+    check(fn(store._pool, layer, _ptr(q), stride[0], _ptr(k), stride[1],
+             _ptr(v), stride[2], _DT[k.dtype], rows, n_heads, _ptr(q_norm),
+             _ptr(k_norm), float(eps), _ptr(positions) if rot else None,
+             _ptr(inv_freq), rot, int(bool(interleaved)), float(attn_factor),
+             _ptr(slot_block), _ptr(slot_off), _ptr(q_out)))
+    return q_out
+
+
 class HipGatherPlan:
     """CudaGatherPlan::new (src/cuda/kv_storage.rs:26-54): each sequence's
     block table padded to max_blocks with its own last block, uploaded once
@@ -491,6 +545,21 @@ class HipKvStorage:
             _ptr(q_norm), _ptr(k_norm), float(eps), _ptr(cos), _ptr(sin),
             _ptr(block_ids), _ptr(offsets), _ptr(q_out)))
         return q_out
+
+    def rope_append(self, layer: int, q, k: torch.Tensor, v: torch.Tensor,
+                    positions, inv_freq, slot_block: torch.Tensor,
+                    slot_off: torch.Tensor, interleaved: bool = False,
+                    attn_factor: float = 1.0, q_norm=None, k_norm=None,
+                    eps: float = 1e-6, q_out=None):
+        """rvkv_rope_append: q and k rotated by their positions (half or
+        interleaved pairs, the first 2 * len(inv_freq) dims), k and v appended
+        at their slots; returns the rotated q. q [rows, n_heads, hd], k and v
+        [rows, n_kv, hd] f32 or f16, rows any stride apart (slices of a fused
+        QKV buffer); inv_freq f32 (rope.rope_inv_freq)."""
+        return rope_append_call(self._L.rvkv_rope_append, self, layer, q, k, v,
+                                positions, inv_freq, slot_block, slot_off,
+                                interleaved, attn_factor, q_norm, k_norm, eps,
+                                q_out)
 
     # -- copy-on-write -------------------------------------------------
     def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor) -> None:
