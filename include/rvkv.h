@@ -632,7 +632,16 @@ int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
  * (larger entries of row_start count as total_rows). q, out: [total_rows,
  * n_heads, head_dim] of dtype, 16-byte aligned; F16 rounds the softmax
  * weights once to f16, F32 is computed to f32 accuracy at about twice the
- * matrix work. Contexts up to 2^32 - 256 tokens. */
+ * matrix work. Contexts up to 2^32 - 256 tokens.
+ * ws: device scratch of at least rvkv_q8_prefill_workspace_bytes(...) bytes,
+ * 256-byte aligned, uninitialised: calls whose rows alone leave the GPU idle
+ * are cut along the keys and merged by a second launch, sized by max_blocks
+ * (pass a table no wider than the longest sequence). NULL: never cut, the same
+ * result to within rounding. Calls that run at once need a ws each. */
+size_t rvkv_q8_prefill_workspace_bytes(const rvkv_q8_pool *pool,
+                                       uint32_t total_rows, uint32_t batch,
+                                       uint32_t n_heads, uint32_t max_blocks,
+                                       int32_t window);
 int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
                            const void *q, rvkv_dtype dtype,
                            const uint32_t *row_start, uint32_t total_rows,
@@ -640,7 +649,8 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
                            const uint32_t *pos_offset,
                            const uint32_t *read_num_tokens, uint32_t batch,
                            uint32_t max_blocks, uint32_t n_heads, float scale,
-                           int32_t window, void *out);
+                           int32_t window, void *out, void *ws,
+                           size_t ws_bytes);
 
 #ifdef __cplusplus
 }

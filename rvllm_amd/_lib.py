@@ -93,7 +93,10 @@ SIGNATURES = {
     "rvkv_q8_paged_decode": (_int, [_P, _u32, _P, _int, _P, _P, _u32, _u32,
                                     _u32, _u32, _f32, _i32, _P, _P, _sz]),
     "rvkv_q8_packed_prefill": (_int, [_P, _u32, _P, _int, _P, _u32, _P, _P, _P,
-                                      _u32, _u32, _u32, _f32, _i32, _P]),
+                                      _u32, _u32, _u32, _f32, _i32, _P, _P,
+                                      _sz]),
+    "rvkv_q8_prefill_workspace_bytes": (_sz, [_P, _u32, _u32, _u32, _u32,
+                                              _i32]),
     "rvkv_sched_last_error": (ctypes.c_char_p, []),
     "rvkv_sched_create": (_P, [_u32, _u32]),
     "rvkv_sched_destroy": (None, [_P]),

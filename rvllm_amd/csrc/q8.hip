@@ -164,7 +164,8 @@ __device__ __forceinline__ half2v pk(float a, float b) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) q8_decode_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
+    q8_decode_kernel(DecodeArgs a) {
   constexpr int NK = HD / 64, NV = HD / 16;
   constexpr float kNone = -__builtin_inff();
   __shared__ float sh_acc[4][8][HD];
@@ -618,7 +619,7 @@ int rvkv_q8_gather(const rvkv_q8_pool *pool, uint32_t layer,
     return fail(RVKV_EINVAL, op, "out dtype must be F16 or F32");
   const uint64_t n = (uint64_t)batch * pool->n_kv * ctx_len *
                      (pool->head_dim / 16);
-  if ((n + 255) / 256 > 0x7fffffffull)
+  if ((n + 255) / 256 > 0xffffffull)
     return fail(RVKV_EUNSUPPORTED, op, "too many rows for one launch");
   const int rc = rvkv_detail::q8_device(op, pool->device);
   if (rc) return rc;

@@ -38,12 +38,24 @@ struct PackedArgs {
   size_t rec;
   uint32_t total_rows, batch, n_heads, n_kv, group, hd, bs, max_blocks;
   uint32_t num_blocks, window;
+  uint32_t n_tiles, n_pieces, piece_keys;
   int32_t bsg_log2;  // log2(bs / 16), -1 if that is no power of two
   float qscale;      // scale * log2(e)
+  float *ws_acc, *ws_ml;
 };
 
 __device__ __forceinline__ half2v pk(float a, float b) {
   return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                                  __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
 }
 
 template <int HD>
@@ -51,81 +63,139 @@ struct Tile {
   // (16 bytes between rows beyond their length: rows on other banks)
   _Float16 k[kKeys][HD + 8];
   _Float16 v[HD][kKeys + 8];
-  float ks[kKeys], vs[kKeys];
-  float vtop[2];
+  float ks[kKeys];  // K scale * scale * log2(e)
+  float vs[kKeys];  // V scale * 2^6 / vnorm; 0 for a key that cannot be read
+  float vnorm;      // a power of two above every V scale so far
+  uint32_t bad;     // bit i: granule i (16 keys) lies in no block
 };
 
+// A workgroup's tile: 128 flattened rows (token * group + head) of one
+// sequence from f0 on, its sequence's fields, and the keys [beg, end) that
+// its rows see.
+struct Work {
+  uint32_t seq, r0, beg, end;
+  uint64_t f0, n_flat, pos0, read;
+};
+
+// Tile t of the launch's index space: sequence b owns indices
+// row_start[b] * group / 128 + b onward, at least as many as it has tiles, so
+// b = (sequences whose first index is at most t) - 1. Every thread of the
+// workgroup calls this; false: no such tile.
+__device__ __forceinline__ bool find_work(const PackedArgs &a, uint32_t t,
+                                          Work &w) {
+  __shared__ uint32_t found[4], field[4];
+  const uint32_t tid = threadIdx.x, G = a.group;
+  uint32_t n = 0, r0 = 0, r1 = 0, pos = 0, read = 0;
+  for (uint32_t b0 = 0; b0 < a.batch; b0 += 256) {
+    const uint32_t b = b0 + tid;
+    bool mine = false;
+    if (b < a.batch) {
+      r0 = a.row_start[b];
+      r1 = a.row_start[b + 1];
+      pos = a.pos_offset[b];
+      read = a.read_num[b];
+      r0 = r0 < a.total_rows ? r0 : a.total_rows;
+      mine = (uint64_t)r0 * G / kRows + b <= t;
+    }
+    n += (uint32_t)__popcll(__ballot(mine));
+  }
+  if ((tid & 63) == 0) found[tid >> 6] = n;
+  __syncthreads();
+  n = found[0] + found[1] + found[2] + found[3];
+  if (n == 0) return false;
+  w.seq = n - 1;
+  if (a.batch <= 256) {  // (this thread holds the sequence's fields)
+    if (tid == w.seq) {
+      field[0] = r0;
+      field[1] = r1;
+      field[2] = pos;
+      field[3] = read;
+    }
+    __syncthreads();
+    r0 = field[0];
+    r1 = field[1];
+    pos = field[2];
+    read = field[3];
+  } else {
+    r0 = a.row_start[w.seq];
+    r1 = a.row_start[w.seq + 1];
+    pos = a.pos_offset[w.seq];
+    read = a.read_num[w.seq];
+  }
+  w.seq = uniform(w.seq);
+  r0 = uniform(r0);
+  r1 = uniform(r1);
+  r0 = r0 < a.total_rows ? r0 : a.total_rows;
+  r1 = r1 < a.total_rows ? r1 : a.total_rows;
+  w.r0 = r0;
+  w.pos0 = uniform(pos);
+  w.n_flat = r1 > r0 ? (uint64_t)(r1 - r0) * G : 0;
+  w.f0 = (uint64_t)(t - (uint32_t)((uint64_t)r0 * G / kRows + w.seq)) * kRows;
+  if (w.f0 >= w.n_flat) return false;
+  // (contexts end below 2^32 - 256, so that no key index wraps)
+  const uint64_t most = (uint64_t)a.max_blocks * a.bs;
+  const uint64_t cap = most < kMaxKeys ? most : kMaxKeys;
+  w.read = uniform(read);
+  w.read = w.read < cap ? w.read : cap;
+  const uint64_t last = w.f0 + kRows < w.n_flat ? w.f0 + kRows - 1
+                                                : w.n_flat - 1;
+  const uint64_t pos_last = w.pos0 + last / G, pos_first = w.pos0 + w.f0 / G;
+  w.end = (uint32_t)(pos_last + 1 < w.read ? pos_last + 1 : w.read);
+  w.beg = 0;
+  if (a.window && pos_first + 1 > a.window)
+    w.beg = (uint32_t)(pos_first + 1 - a.window < w.read
+                           ? pos_first + 1 - a.window : w.read);
+  w.beg &= ~15u;
+  return true;
+}
+
 template <typename T, int HD, bool SPLIT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     q8_prefill_kernel(PackedArgs a) {
   constexpr int NC = HD / 16, ND = HD / 32;
   constexpr int KPT = HD / 64;  // 16-byte chunks of K, and of V, a thread
   constexpr float kNone = -__builtin_inff();
   extern __shared__ __align__(16) unsigned char smem[];
   Tile<HD> *tiles = reinterpret_cast<Tile<HD> *>(smem);
-  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const uint32_t col = lane & 31, h = lane >> 5;
-  const uint32_t G = a.group, kvh = blockIdx.y, hd = a.hd, bs = a.bs;
-
-  // The tile index space: sequence b owns row_start[b] * G / 128 + b onward,
-  // at least as many as it has tiles. b = (sequences that start at or before
-  // this index) - 1.
-  const uint32_t t = gridDim.x - 1 - blockIdx.x;
-  uint32_t seq, local;
-  {
-    __shared__ uint32_t count;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    uint32_t n = 0;
-    for (uint32_t b = tid; b < a.batch; b += 256) {
-      const uint32_t r = a.row_start[b] < a.total_rows ? a.row_start[b]
-                                                       : a.total_rows;
-      n += (uint64_t)r * G / kRows + b <= t ? 1 : 0;
+  const uint32_t G = a.group, hd = a.hd, bs = a.bs, bsg = bs / 16;
+  // KV heads innermost: the tiles of one head share an XCD's L2 where their
+  // number is a multiple of eight. The last tiles, which see most, first.
+  const uint32_t kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
+  const uint32_t piece = rest % a.n_pieces;
+  const uint32_t t = a.n_tiles - 1 - rest / a.n_pieces;
+  Work w;
+  if (!find_work(a, t, w)) return;
+  uint32_t beg = w.beg, end = w.end;
+  bool whole = true;  // this workgroup sees all its rows' keys
+  if (a.n_pieces > 1) {
+    whole = end <= beg || end - beg <= a.piece_keys;
+    if (whole) {
+      if (piece) return;
+    } else {
+      const uint64_t from = (uint64_t)beg + (uint64_t)piece * a.piece_keys;
+      if (from >= end) return;
+      beg = (uint32_t)from;
+      if (end - beg > a.piece_keys) end = beg + a.piece_keys;
     }
-    if (n) atomicAdd(&count, n);  // (a whole number: any order)
-    __syncthreads();
-    if (count == 0) return;
-    seq = count - 1;
   }
-  uint32_t r0 = a.row_start[seq], r1 = a.row_start[seq + 1];
-  r0 = r0 < a.total_rows ? r0 : a.total_rows;
-  r1 = r1 < a.total_rows ? r1 : a.total_rows;
-  local = t - (uint32_t)((uint64_t)r0 * G / kRows + seq);
-  const uint64_t n_flat = r1 > r0 ? (uint64_t)(r1 - r0) * G : 0;
-  const uint64_t f0 = (uint64_t)local * kRows;
-  if (f0 >= n_flat) return;
 
-  // (contexts end below 2^32 - 256, so that no key index wraps)
-  const uint64_t most = (uint64_t)a.max_blocks * bs;
-  const uint64_t cap = most < kMaxKeys ? most : kMaxKeys;
-  uint64_t read = a.read_num[seq];
-  read = read < cap ? read : cap;
-  const uint64_t pos0 = a.pos_offset[seq];
   // This lane's q row, and the keys [key_lo, key_hi) that it sees.
-  const uint64_t f = f0 + wave * 32 + col;
-  const bool live = f < n_flat;
-  const uint32_t tok = (uint32_t)((live ? f : f0) / G);
-  const uint32_t head = kvh * G + (uint32_t)((live ? f : f0) % G);
-  const size_t row = ((size_t)(r0 + tok) * a.n_heads + head) * hd;
-  const uint64_t pos = pos0 + tok;
-  uint32_t key_hi = (uint32_t)(pos + 1 < read ? pos + 1 : read);
+  const uint64_t f = w.f0 + wave * 32 + col;
+  const bool live = f < w.n_flat;
+  const uint32_t tok = (uint32_t)((live ? f : w.f0) / G);
+  const uint32_t head = kvh * G + (uint32_t)((live ? f : w.f0) % G);
+  const size_t row = ((size_t)(w.r0 + tok) * a.n_heads + head) * hd;
+  const uint64_t pos = w.pos0 + tok;
+  uint32_t key_hi = (uint32_t)(pos + 1 < w.read ? pos + 1 : w.read);
   uint32_t key_lo = a.window && pos + 1 > a.window
-                        ? (uint32_t)(pos + 1 - a.window < read
-                                         ? pos + 1 - a.window : read) : 0;
+                        ? (uint32_t)(pos + 1 - a.window < w.read
+                                         ? pos + 1 - a.window : w.read) : 0;
   if (!live) key_hi = key_lo = 0;
-  // The workgroup's keys: those of its first and last row.
-  const uint64_t last = f0 + kRows < n_flat ? f0 + kRows - 1 : n_flat - 1;
-  const uint64_t pos_last = pos0 + last / G, pos_first = pos0 + f0 / G;
-  const uint32_t end = (uint32_t)(pos_last + 1 < read ? pos_last + 1 : read);
-  uint32_t beg = 0;
-  if (a.window && pos_first + 1 > a.window)
-    beg = (uint32_t)(pos_first + 1 - a.window < read
-                         ? pos_first + 1 - a.window : read);
-  beg &= ~15u;
   // Keys that every row of this wave sees, and that any does.
   uint32_t all_lo = key_lo, all_hi = live ? key_hi : 0xffffffffu,
-           any_hi = key_hi;
-  uint32_t any_lo = live ? key_lo : 0xffffffffu;
+           any_hi = key_hi, any_lo = live ? key_lo : 0xffffffffu;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) {
     all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, o));
@@ -133,10 +203,118 @@ __global__ void __launch_bounds__(256)
     any_hi = max(any_hi, (uint32_t)__shfl_xor((int)any_hi, o));
     any_lo = min(any_lo, (uint32_t)__shfl_xor((int)any_lo, o));
   }
+  all_lo = uniform(all_lo);
+  all_hi = uniform(all_hi);
+  any_lo = uniform(any_lo);
+  any_hi = uniform(any_hi);
 
-  // q: element j of chunk c is dim 16 c + 8 h + j.
+  const uint32_t *table = a.tables + (size_t)w.seq * a.max_blocks;
+  const uint32_t last_granule = w.end ? (w.end - 1) / 16 : 0;
+  // A granule's record and place in it (granules behind the last are not
+  // looked up: their keys are masked).
+  struct Place {
+    uint32_t blk, in;
+  };
+  const auto place = [&](uint32_t x) {
+    x = x < last_granule ? x : last_granule;
+    Place p;
+    const uint32_t bi = a.bsg_log2 >= 0 ? x >> a.bsg_log2 : x / bsg;
+    p.in = x - bi * bsg;
+    p.blk = table[bi];
+    return p;
+  };
+  // K chunk i of a thread: key (tid + 256 i) / NC, in a granule that is the
+  // wave's (its lanes' keys lie in one).
+  const uint32_t k_key = tid / NC, k_ch = tid % NC;
+  constexpr int kStep = 256 / NC;  // keys from one chunk to the next
+  const uint32_t gv = tid & 3, vd = tid >> 2;
+  Place kp[KPT], vp, sp;
+  const auto look_up = [&](uint32_t kt) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      kp[i] = place(kt / 16 + uniform((k_key + kStep * i) >> 4));
+    vp = place(kt / 16 + gv);
+    sp = place(kt / 16 + (lane >> 4));
+  };
+  uint4 kraw[KPT], vraw[KPT];
+  float sraw = 0.f;
+  bool unread = false;
+  const size_t head_at = (size_t)kvh * bs * hd;
+  const unsigned char *scale_at =
+      (wave == 0 ? a.kc : a.vc) + (size_t)a.n_kv * bs * hd +
+      ((size_t)kvh * bs + (lane & 15)) * 4;
+  const auto fetch = [&](uint32_t kt) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const uint32_t kb = kp[i].blk < a.num_blocks ? kp[i].blk : 0;
+      kraw[i] = uint4{};
+      if (k_ch * 16 < hd)
+        kraw[i] = *reinterpret_cast<const uint4 *>(
+            a.kc + kb * a.rec + head_at +
+            (kp[i].in * 16 + ((k_key + kStep * i) & 15)) * hd + k_ch * 16);
+    }
+    const uint32_t vb = vp.blk < a.num_blocks ? vp.blk : 0;
+    const unsigned char *v0 = a.vc + vb * a.rec + head_at + vp.in * 16;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      vraw[i] = uint4{};
+      if (vd + 64 * i < hd)
+        vraw[i] = *reinterpret_cast<const uint4 *>(v0 + (vd + 64 * i) * bs);
+    }
+    if (wave < 2) {
+      unread = sp.blk >= a.num_blocks;
+      sraw = 0.f;
+      if (!unread && kt + lane < end)
+        sraw = *reinterpret_cast<const float *>(scale_at + sp.blk * a.rec +
+                                                sp.in * 64);
+    }
+  };
+  float v_so_far = kVnorm0;  // (wave 1's)
+  const auto put = [&](Tile<HD> &s) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      half8v *k = reinterpret_cast<half8v *>(&s.k[k_key + kStep * i][k_ch * 16]);
+      k[0] = codes_to_half8(kraw[i].x, kraw[i].y);
+      k[1] = codes_to_half8(kraw[i].z, kraw[i].w);
+    }
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      half8v *v = reinterpret_cast<half8v *>(&s.v[vd + 64 * i][gv * 16]);
+      v[0] = codes_to_half8(vraw[i].x, vraw[i].y);
+      v[1] = codes_to_half8(vraw[i].z, vraw[i].w);
+    }
+    if (wave == 0) {
+      s.ks[lane] = sraw * a.qscale;
+      const uint64_t b = __ballot(unread);
+      if (lane == 0)
+        s.bad = (uint32_t)((b & 1) | (b >> 15 & 2) | (b >> 30 & 4) |
+                           (b >> 45 & 8));
+    } else if (wave == 1) {
+      float top = sraw;
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      if (top >= v_so_far) {
+        uint32_t e = (__float_as_uint(top) >> 23) + 1;
+        e = e > 253 ? 253 : e;
+        v_so_far = __uint_as_float(e << 23);
+      }
+      s.vs[lane] =
+          sraw * __uint_as_float((260u << 23) - __float_as_uint(v_so_far));
+      if (lane == 0) s.vnorm = v_so_far;
+    }
+  };
+
+  const bool any = beg < end;
+  if (any) {
+    look_up(beg);
+    fetch(beg);
+    look_up(beg + kKeys);
+  }
+
+  // q: element j of chunk c is dim 16 c + 8 h + j. rf: what a score is still
+  // to be multiplied by.
   half8v qh[NC], ql[SPLIT ? NC : 1];
-  float qscale = a.qscale;
+  float rf = 1.f;
   {
     const T *q = (const T *)a.q + row;
     if constexpr (!SPLIT) {
@@ -148,257 +326,199 @@ __global__ void __launch_bounds__(256)
     } else {
       // (brought just below 2^15 by a power of two: neither part leaves f16's
       // range, the lower one not its normal numbers)
+      float x[NC][8];
       float top = 0.f;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (live && (uint32_t)c * 16 < hd)
-            top = fmaxf(top, fabsf((float)q[c * 16 + 8 * h + j]));
-      top = fmaxf(top, __shfl_xor(top, 32));
+        for (int j = 0; j < 8; ++j) {
+          x[c][j] = live && (uint32_t)c * 16 < hd
+                        ? (float)q[c * 16 + 8 * h + j] : 0.f;
+          top = fmaxf(top, fabsf(x[c][j]));
+        }
+      top = max_halves(top);
       const uint32_t ex = scale_exponent(top);
       const float down = __uint_as_float((269 - ex) << 23);
-      qscale *= __uint_as_float((ex - 15) << 23);
+      rf = __uint_as_float((ex - 15) << 23);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = live && (uint32_t)c * 16 < hd
-                              ? (float)q[c * 16 + 8 * h + j] * down : 0.f;
+          const float y = x[c][j] * down;
           qh[c][j] = (_Float16)y;
           ql[c][j] = (_Float16)(y - (float)qh[c][j]);
         }
     }
   }
 
-  const uint32_t *table = a.tables + (size_t)seq * a.max_blocks;
-  const uint32_t last_granule = end ? (end - 1) / 16 : 0;
-  // The records of a tile's four granules of 16 keys (uniform).
-  struct Places {
-    uint32_t blk[4], in[4];
-  };
-  const auto places = [&](uint32_t kt) {
-    Places p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t x = kt / 16 + i;
-      x = x < last_granule ? x : last_granule;
-      const uint32_t bi = a.bsg_log2 >= 0 ? x >> a.bsg_log2 : x / (bs / 16);
-      p.in[i] = x - bi * (bs / 16);
-      p.blk[i] = table[bi];
-    }
-    return p;
-  };
-  const auto pick = [](const uint32_t (&x)[4], uint32_t i) {
-    return i & 2 ? (i & 1 ? x[3] : x[2]) : (i & 1 ? x[1] : x[0]);
-  };
-  uint4 kraw[KPT], vraw[KPT];
-  float sraw;
-  const auto fetch = [&](uint32_t kt, const Places &p) {
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const uint32_t x = tid + 256 * i;
-      const uint32_t key = x / NC, ch = x % NC, gr = key / 16;
-      uint32_t blk = pick(p.blk, gr);
-      blk = blk < a.num_blocks ? blk : 0;
-      kraw[i] = uint4{};
-      if (ch * 16 < hd)
-        kraw[i] = *reinterpret_cast<const uint4 *>(
-            a.kc + blk * a.rec + (size_t)kvh * bs * hd +
-            (pick(p.in, gr) * 16 + key % 16) * hd + ch * 16);
-      const uint32_t d = x / 4, gv = x % 4;
-      blk = pick(p.blk, gv);
-      blk = blk < a.num_blocks ? blk : 0;
-      vraw[i] = uint4{};
-      if (d < hd)
-        vraw[i] = *reinterpret_cast<const uint4 *>(
-            a.vc + blk * a.rec + (size_t)kvh * bs * hd + (size_t)d * bs +
-            pick(p.in, gv) * 16);
-    }
-    // Scales: threads 0-63 K's, 64-127 V's; 0 where the key cannot be read.
-    if (tid < 128) {
-      const uint32_t key = tid & 63, gr = key / 16;
-      const uint32_t blk = pick(p.blk, gr);
-      const bool ok = blk < a.num_blocks && kt + key < end;
-      sraw = ok ? *reinterpret_cast<const float *>(
-                      (tid < 64 ? a.kc : a.vc) + blk * a.rec +
-                      (size_t)a.n_kv * bs * hd +
-                      ((size_t)kvh * bs + pick(p.in, gr) * 16 + key % 16) * 4)
-                : 0.f;
-    }
-  };
-  const auto put = [&](Tile<HD> &s) {
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const uint32_t x = tid + 256 * i;
-      half8v *k = reinterpret_cast<half8v *>(&s.k[x / NC][x % NC * 16]);
-      k[0] = codes_to_half8(kraw[i].x, kraw[i].y);
-      k[1] = codes_to_half8(kraw[i].z, kraw[i].w);
-      half8v *v = reinterpret_cast<half8v *>(&s.v[x / 4][x % 4 * 16]);
-      v[0] = codes_to_half8(vraw[i].x, vraw[i].y);
-      v[1] = codes_to_half8(vraw[i].z, vraw[i].w);
-    }
-    if (tid < 64) s.ks[tid] = sraw;
-    if (tid >= 64 && tid < 128) {
-      s.vs[tid - 64] = sraw;
-      float top = sraw;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-      if (tid == 64) s.vtop[0] = top;
-    }
-  };
-
+  // m: what the weights are relative to, their maximum to within 2^8 (it
+  // moves, and o and l with it, only when a score passes it by more).
   float m = kNone, l = 0.f;
-  float vnorm = kVnorm0;  // power of two above every vs
+  float vnorm = kVnorm0;
   float16v o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = float16v{};
+  const uint32_t key_row = 16 * (col >> 4) + 8 * ((col >> 2) & 1) +
+                           4 * ((col >> 3) & 1) + (col & 3);
 
-  if (beg < end) {
-    Places p = places(beg);
-    fetch(beg, p);
-    put(tiles[0]);
-    uint32_t bad = 0;  // granules of the current tile that cannot be read
+  const auto step = [&](const Tile<HD> &s, uint32_t kt) {
+    float16v sc[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (p.blk[i] >= a.num_blocks) << i;
-    p = places(beg + kKeys);
+    for (int kh = 0; kh < 2; ++kh) {
+      sc[kh] = float16v{};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const half8v kf = *reinterpret_cast<const half8v *>(
+            &s.k[kh * 32 + key_row][c * 16 + 8 * h]);
+        sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[c], sc[kh], 0,
+                                                        0, 0);
+        if constexpr (SPLIT)
+          sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[c], sc[kh],
+                                                          0, 0, 0);
+      }
+    }
+    // Register 8 u + j of half kh: key 32 kh + 16 u + 8 h + j.
+    float top = kNone;
+    const uint32_t bad = uniform(s.bad);
+    const bool masked = kt < all_lo || kt + kKeys > all_hi || bad;
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float4v k4 = *reinterpret_cast<const float4v *>(
+            &s.ks[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[kh][r + i] *= k4[i];
+      }
+    if (masked) {  // (uniform over the wave)
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t key = kt + kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7);
+          const bool ok = key >= key_lo && key < key_hi &&
+                          !(bad >> (2 * kh + (r >> 3)) & 1);
+          sc[kh][r] = ok ? sc[kh][r] : kNone;
+        }
+    }
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        top = fmaxf(fmaxf(sc[kh][r], sc[kh][r + 1]), top);
+    top = max_halves(top);
+    if constexpr (SPLIT) top *= rf;
+    float fix = 1.f;
+    if (__any(top > m + 8.f)) {
+      const float now = fmaxf(m, top);
+      // (-inf less -inf: nothing was seen, and nothing is held)
+      fix = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= fix;
+    }
+    if (s.vnorm != vnorm) {  // (uniform)
+      fix *= vnorm / s.vnorm;
+      vnorm = s.vnorm;
+    }
+    if (__any(fix != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= fix;
+    }
+    const float mm = m == kNone ? 0.f : m;
+    half8v ph[4], pl[SPLIT ? 4 : 1];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float4v v4 = *reinterpret_cast<const float4v *>(
+            &s.vs[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
+        half8v &up = ph[2 * kh + (r >> 3)];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          float y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = __builtin_amdgcn_exp2f(
+                SPLIT ? __builtin_fmaf(sc[kh][r + i + e], rf, -mm)
+                      : sc[kh][r + i + e] - mm);
+            l += x;
+            // (0 for a key that is left out, whatever its scale holds)
+            y[e] = rvkv_mul0(x, v4[i + e]);
+          }
+          const int at = (r & 7) + i;
+          if constexpr (SPLIT) {
+            half8v &lo = pl[2 * kh + (r >> 3)];
+            const half2v u = pk(y[0], y[1]);
+            const half2v v = pk(y[0] - (float)u[0], y[1] - (float)u[1]);
+            up[at] = u[0];
+            up[at + 1] = u[1];
+            lo[at] = v[0];
+            lo[at + 1] = v[1];
+          } else {
+            up[at] = (_Float16)y[0];
+            up[at + 1] = (_Float16)y[1];
+          }
+        }
+      }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      if ((uint32_t)d * 32 < hd) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const half8v vf = *reinterpret_cast<const half8v *>(
+              &s.v[d * 32 + col][x * 16 + 8 * h]);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[x], o[d], 0, 0,
+                                                        0);
+          if constexpr (SPLIT)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[x], o[d], 0,
+                                                          0, 0);
+        }
+      }
+  };
+
+  if (any) {
+    put(tiles[0]);
     __syncthreads();
     uint32_t buf = 0;
-    for (uint32_t kt = beg; kt < end; kt += kKeys, buf ^= 1) {
-      const Tile<HD> &s = tiles[buf];
+    for (uint32_t kt = beg;; kt += kKeys, buf ^= 1) {
       const bool more = end - kt > kKeys;
-      uint32_t bad_next = 0;
       if (more) {
-        fetch(kt + kKeys, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bad_next |= (p.blk[i] >= a.num_blocks) << i;
-        p = places(kt + 2 * kKeys);
+        fetch(kt + kKeys);
+        look_up(kt + 2 * kKeys);
       }
-      if (kt < any_hi && kt + kKeys > any_lo) {  // (uniform over the wave)
-        float16v sc[2];
-        const uint32_t key_row = 16 * (col >> 4) + 8 * ((col >> 2) & 1) +
-                                 4 * ((col >> 3) & 1) + (col & 3);
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          sc[kh] = float16v{};
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const half8v kf = *reinterpret_cast<const half8v *>(
-                &s.k[kh * 32 + key_row][c * 16 + 8 * h]);
-            sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[c], sc[kh],
-                                                            0, 0, 0);
-            if constexpr (SPLIT)
-              sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[c],
-                                                              sc[kh], 0, 0, 0);
-          }
-        }
-        // Result register 8 u + j of half kh: key 32 kh + 16 u + 8 h + j.
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            const float4v k4 = *reinterpret_cast<const float4v *>(
-                &s.ks[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sc[kh][r + i] *= k4[i] * qscale;
-          }
-        if (kt < all_lo || kt + kKeys > all_hi || bad) {
-#pragma unroll
-          for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const uint32_t key = kt + kh * 32 + 16 * (r >> 3) + 8 * h +
-                                   (r & 7);
-              const bool ok = key >= key_lo && key < key_hi &&
-                              !(bad >> (2 * kh + (r >> 3)) & 1);
-              sc[kh][r] = ok ? sc[kh][r] : kNone;
-            }
-        }
-        float top = sc[0][0];
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[kh][r]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m, top);
-        const float mm = m_new == kNone ? 0.f : m_new;
-        float fix = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - mm);
-        m = m_new;
-        l *= fix;
-        const float vtop = s.vtop[0];
-        if (vtop >= vnorm) {  // (uniform)
-          uint32_t e = (__float_as_uint(vtop) >> 23) + 1;
-          e = e > 253 ? 253 : e;
-          const float now = __uint_as_float(e << 23);
-          fix *= vnorm / now;
-          vnorm = now;
-        }
-        if (!__all(fix == 1.f)) {
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[d] *= fix;
-        }
-        // (weights up to 2^15, as q)
-        const float vdown =
-            __uint_as_float((269u << 23) - __float_as_uint(vnorm));
-        half8v ph[4], pl[SPLIT ? 4 : 1];
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            const float4v v4 = *reinterpret_cast<const float4v *>(
-                &s.vs[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = __builtin_amdgcn_exp2f(sc[kh][r + i] - mm);
-              l += x;
-              // (0 for a key that is left out, whatever its scale holds)
-              w[i] = rvkv_mul0(x, v4[i] * vdown);
-            }
-            half8v &up = ph[2 * kh + (r >> 3)];
-            if constexpr (SPLIT) {
-              half8v &lo = pl[2 * kh + (r >> 3)];
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const half2v x = pk(w[i], w[i + 1]);
-                const half2v y = pk(w[i] - (float)x[0],
-                                    w[i + 1] - (float)x[1]);
-                up[(r & 7) + i] = x[0];
-                up[(r & 7) + i + 1] = x[1];
-                lo[(r & 7) + i] = y[0];
-                lo[(r & 7) + i + 1] = y[1];
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) up[(r & 7) + i] = (_Float16)w[i];
-            }
-          }
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-          if ((uint32_t)d * 32 < hd) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const half8v vf = *reinterpret_cast<const half8v *>(
-                  &s.v[d * 32 + col][x * 16 + 8 * h]);
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[x], o[d], 0,
-                                                            0, 0);
-              if constexpr (SPLIT)
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[x], o[d],
-                                                              0, 0, 0);
-            }
-          }
-      }
-      if (more) put(tiles[buf ^ 1]);
-      bad = bad_next;
+      if (kt < any_hi && kt + kKeys > any_lo) step(tiles[buf], kt);
+      if (!more) break;
+      put(tiles[buf ^ 1]);
       __syncthreads();
     }
   }
 
   l += __shfl_xor(l, 32);
+  const float back = vnorm * 0x1p-6f;
+  if (!whole) {
+    // A piece's part: o and l relative to m, for the merge.
+    const size_t slot =
+        ((size_t)(t * a.n_kv + kvh) * a.n_pieces + piece) * kRows + wave * 32 +
+        col;
+    float *to = a.ws_acc + slot * HD;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        float4v y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = o[d][r + i] * back;
+        *reinterpret_cast<float4v *>(to + d * 32 + 2 * r + 4 * h) = y;
+      }
+    if (h == 0) {
+      a.ws_ml[2 * slot] = m;
+      a.ws_ml[2 * slot + 1] = l;
+    }
+    return;
+  }
   if (!live) return;
   T *out = (T *)a.out + row;
-  const float inv = l == 0.f ? 0.f : vnorm * 0x1p-15f / l;
+  const float inv = l == 0.f ? 0.f : back / l;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -414,6 +534,86 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// Merges the pieces of tiles that were cut: 32 rows a workgroup, HD / 4
+// threads a row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) q8_prefill_reduce_kernel(PackedArgs a) {
+  constexpr float kNone = -__builtin_inff();
+  constexpr uint32_t TR = HD / 4;
+  const uint32_t kvh = blockIdx.x % a.n_kv, t = blockIdx.x / a.n_kv;
+  Work w;
+  if (!find_work(a, t, w)) return;
+  if (w.end <= w.beg || w.end - w.beg <= a.piece_keys) return;
+  const uint32_t live = (w.end - w.beg - 1) / a.piece_keys + 1;
+  const uint32_t d = threadIdx.x % TR * 4;
+  for (uint32_t r = threadIdx.x / TR; r < 32; r += 256 / TR) {
+    const uint32_t in = blockIdx.y * 32 + r;
+    const uint64_t f = w.f0 + in;
+    if (f >= w.n_flat) return;
+    const size_t slot0 = (size_t)(t * a.n_kv + kvh) * a.n_pieces * kRows + in;
+    float top = kNone;
+    for (uint32_t p = 0; p < live; ++p)
+      top = fmaxf(top, a.ws_ml[2 * (slot0 + p * kRows)]);
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (uint32_t p = 0; p < live; ++p) {
+      const size_t slot = slot0 + p * kRows;
+      const float m = a.ws_ml[2 * slot];
+      const float e = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      l += a.ws_ml[2 * slot + 1] * e;
+      o += *reinterpret_cast<const float4v *>(a.ws_acc + slot * HD + d) * e;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t tok = (uint32_t)(f / a.group);
+    const uint32_t head = kvh * a.group + (uint32_t)(f % a.group);
+    if (d < a.hd) {
+      T *out = (T *)a.out + ((size_t)(w.r0 + tok) * a.n_heads + head) * a.hd;
+      typedef T vec4 __attribute__((ext_vector_type(4)));
+      vec4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = (T)(o[i] * inv);
+      *reinterpret_cast<vec4 *>(out + d) = y;
+    }
+  }
+}
+
+uint32_t hd_up(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+
+struct Layout {
+  uint64_t n_tiles, n_pieces, piece_keys;
+  size_t ml_off, bytes;
+};
+
+// How a call is cut. The rows' tiles alone where they give every CU its
+// workgroups (two up to hd 128, one above); otherwise each tile's keys, as far
+// as the host can tell them from the width of the table and the window, in
+// pieces of at least 128.
+Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
+              uint32_t n_heads, uint32_t max_blocks, uint32_t window) {
+  Layout w{};
+  const uint32_t G = n_heads / p->n_kv;
+  w.n_tiles = (uint64_t)total_rows * G / kRows + batch;
+  w.n_pieces = 1;
+  uint64_t keys = (uint64_t)max_blocks * p->block_size;
+  if (keys > kMaxKeys) keys = kMaxKeys;
+  const uint64_t band = (uint64_t)window + kRows / G + 16;
+  if (window && band < keys) keys = band;
+  w.piece_keys = keys;
+  const uint64_t have = w.n_tiles * p->n_kv;
+  const uint64_t want = p->head_dim > 128 ? 256 : 512;
+  if (have == 0 || have * 2 > want) return w;
+  uint64_t n = want / have;
+  if (n > (keys + 127) / 128) n = (keys + 127) / 128;
+  if (n > 16) n = 16;
+  if (n < 2) return w;
+  w.piece_keys = ((keys + n - 1) / n + kKeys - 1) / kKeys * kKeys;
+  w.n_pieces = (keys + w.piece_keys - 1) / w.piece_keys;
+  const size_t rows = (size_t)have * w.n_pieces * kRows;
+  w.ml_off = rows * hd_up(p->head_dim) * 4;
+  w.bytes = (w.ml_off + rows * 8 + 255) & ~(size_t)255;
+  return w;
+}
+
 template <typename T, int HD, bool SPLIT>
 int launch(const char *op, const PackedArgs &a, hipStream_t st) {
   const size_t lds = 2 * sizeof(Tile<HD>);
@@ -421,11 +621,13 @@ int launch(const char *op, const PackedArgs &a, hipStream_t st) {
       reinterpret_cast<const void *>(&q8_prefill_kernel<T, HD, SPLIT>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (set != hipSuccess) return hip_fail(op, set);
-  const uint64_t tiles = (uint64_t)a.total_rows * a.group / kRows + a.batch;
-  if (tiles > 0x7fffffffull)
-    return fail(RVKV_EUNSUPPORTED, op, "too many rows for one launch");
   hipLaunchKernelGGL((q8_prefill_kernel<T, HD, SPLIT>),
-                     dim3((uint32_t)tiles, a.n_kv), dim3(256), lds, st, a);
+                     dim3(a.n_tiles * a.n_kv * a.n_pieces), dim3(256), lds, st,
+                     a);
+  if (a.n_pieces > 1)
+    hipLaunchKernelGGL((q8_prefill_reduce_kernel<T, HD>),
+                       dim3(a.n_tiles * a.n_kv, kRows / 32), dim3(256), 0, st,
+                       a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
 }
@@ -441,6 +643,15 @@ int launch(const char *op, const PackedArgs &a, hipStream_t st) {
 
 extern "C" {
 
+size_t rvkv_q8_prefill_workspace_bytes(const rvkv_q8_pool *pool,
+                                       uint32_t total_rows, uint32_t batch,
+                                       uint32_t n_heads, uint32_t max_blocks,
+                                       int32_t window) {
+  if (!pool || n_heads == 0 || n_heads % pool->n_kv) return 0;
+  return layout(pool, total_rows, batch, n_heads, max_blocks,
+                window > 0 ? (uint32_t)window : 0).bytes;
+}
+
 int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
                            const void *q, rvkv_dtype dtype,
                            const uint32_t *row_start, uint32_t total_rows,
@@ -448,7 +659,8 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
                            const uint32_t *pos_offset,
                            const uint32_t *read_num_tokens, uint32_t batch,
                            uint32_t max_blocks, uint32_t n_heads, float scale,
-                           int32_t window, void *out) {
+                           int32_t window, void *out, void *ws,
+                           size_t ws_bytes) {
   const char *op = "packed_prefill";
   if (!pool) return fail(RVKV_EINVAL, op, "pool is NULL");
   if (layer >= pool->n_layers)
@@ -468,6 +680,16 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
   if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
     return fail(RVKV_EINVAL, op, "q and out must be 16-byte aligned");
   const uint32_t bsg = pool->block_size / 16;
+  const uint32_t win = window > 0 ? (uint32_t)window : 0;
+  Layout w = layout(pool, total_rows, batch, n_heads, max_blocks, win);
+  if (!ws) w.n_pieces = 1;
+  if (w.n_pieces > 1 && ws_bytes < w.bytes)
+    return fail(RVKV_EINVAL, op, "workspace smaller than the required bytes");
+  if ((uintptr_t)ws % 256)
+    return fail(RVKV_EINVAL, op, "workspace must be 256-byte aligned");
+  // (a launch holds fewer than 2^32 threads)
+  if (w.n_tiles > 0xffffffu || w.n_tiles * pool->n_kv * w.n_pieces > 0xffffffu)
+    return fail(RVKV_EUNSUPPORTED, op, "too many rows for one launch");
   const int rc = rvkv_detail::q8_device(op, pool->device);
   if (rc) return rc;
   PackedArgs a{};
@@ -489,7 +711,12 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
   a.bs = pool->block_size;
   a.max_blocks = max_blocks;
   a.num_blocks = pool->num_blocks;
-  a.window = window > 0 ? (uint32_t)window : 0;
+  a.window = win;
+  a.n_tiles = (uint32_t)w.n_tiles;
+  a.n_pieces = (uint32_t)w.n_pieces;
+  a.piece_keys = (uint32_t)w.piece_keys;
+  a.ws_acc = static_cast<float *>(ws);
+  a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.ml_off);
   a.bsg_log2 = bsg & (bsg - 1) ? -1 : __builtin_ctz(bsg);
   a.qscale = scale * kLog2e;
   return dtype == RVKV_F16 ? launch<_Float16, false>(op, a, pool->stream)

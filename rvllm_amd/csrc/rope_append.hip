@@ -315,7 +315,7 @@ int rope_append(const char *op, int cell, hipStream_t st, RopeArgs &a,
     return fail(RVKV_EUNSUPPORTED, op, "head_dim must be at most 256");
   if (interleaved > 1)
     return fail(RVKV_EINVAL, op, "interleaved must be 0 or 1");
-  if (a.rows > 0x7fffffffu)
+  if (a.rows > 0xffffffu)  // (a launch holds fewer than 2^32 threads)
     return fail(RVKV_EUNSUPPORTED, op, "too many rows for one launch");
   const uint64_t kv_row = (uint64_t)a.n_kv * a.hd;
   if (a.rows > 1 && (a.k_stride < kv_row || a.v_stride < kv_row ||

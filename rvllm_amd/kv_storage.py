@@ -45,57 +45,73 @@ def _dev_u32(x, device) -> torch.Tensor:
     return torch.from_numpy(arr.copy()).to(device)
 
 
+def _on(store, op: str, tensors) -> None:
+    for t in tensors:
+        if t.device != store.device:
+            raise RvkvError(f"{op}: every tensor must be on the storage's "
+                            "device")
+
+
+def _rows_of(op: str, name: str, t, rows: int, hd: int, dtype) -> int:
+    """Checks a [rows, heads, head_dim] input; its elements between rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != rows or shape[2] != hd:
+        raise RvkvError(f"{op}: {name} must be [rows, heads, head_dim]")
+    if t.dtype != dtype:
+        raise RvkvError(f"{op}: q/k/v must all be float32 or float16")
+    # (the stride of a dimension of size 1 is of no account)
+    if (stride[2] != 1 and hd != 1) or (stride[1] != hd and shape[1] != 1):
+        raise RvkvError(f"{op}: a row's heads must lie one behind the other")
+    return stride[0] if rows > 1 else shape[1] * hd
+
+
 def rope_append_call(fn, store, layer: int, q, k, v, positions, inv_freq,
                      slot_block, slot_off, interleaved, attn_factor, q_norm,
                      k_norm, eps, q_out):
     """rvkv_rope_append / rvkv_q8_rope_append (fn) with what the C ABI cannot
     see checked first. q None: no query heads; inv_freq None: no rotation."""
-    hd, kv = store.head_dim, store.n_kv_heads
     op = "rope_append"
-    rows = int(k.shape[0])
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t is None and name == "q":
-            continue
-        _need(t.dim() == 3 and t.shape[0] == rows and t.shape[2] == hd and
-              (name == "q" or t.shape[1] == kv),
-              f"{op}: {name} must be [rows, heads, head_dim]")
-        _need(t.dtype == k.dtype and t.dtype in _DT,
-              f"{op}: q/k/v must all be float32 or float16")
-        # (the stride of a dimension of size 1 is of no account)
-        _need((hd == 1 or t.stride(2) == 1) and
-              (t.shape[1] == 1 or t.stride(1) == hd),
-              f"{op}: a row's heads must lie one behind the other")
-    n_heads = 0 if q is None else int(q.shape[1])
-    rot = 0 if inv_freq is None else 2 * int(inv_freq.numel())
-    ints = [slot_block, slot_off] + ([positions] if rot else [])
+    hd, kv, dtype, rows = (store.head_dim, store.n_kv_heads, k.dtype,
+                           int(k.shape[0]))
+    _need(dtype in _DT, f"{op}: q/k/v must all be float32 or float16")
+    ks = _rows_of(op, "k", k, rows, hd, dtype)
+    vs = _rows_of(op, "v", v, rows, hd, dtype)
+    _need(k.shape[1] == kv and v.shape[1] == kv,
+          f"{op}: k and v must be [rows, n_kv_heads, head_dim]")
+    used = [k, v, slot_block, slot_off]
+    qs = n_heads = rot = 0
+    if q is not None:
+        qs, n_heads = _rows_of(op, "q", q, rows, hd, dtype), int(q.shape[1])
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        elif (q_out.shape != q.shape or q_out.dtype != dtype or
+              not q_out.is_contiguous()):
+            raise RvkvError(f"{op}: q_out must be contiguous and match q")
+        used += [q, q_out]
+    ints = [slot_block, slot_off]
+    if inv_freq is not None:
+        rot = 2 * int(inv_freq.numel())
+        _need(inv_freq.dtype == torch.float32 and inv_freq.is_contiguous(),
+              f"{op}: inv_freq must be contiguous float32")
+        used += [inv_freq, positions]
+        ints.append(positions)
     for t in ints:
-        _need(t.numel() == rows and t.dtype == torch.int32 and
-              t.is_contiguous(),
-              f"{op}: positions/block_ids/offsets must be contiguous int32, "
-              "one per row")
-    floats = [(inv_freq, None), (q_norm, hd), (k_norm, hd)]
-    for t, n in floats:
-        _need(t is None or (t.dtype == torch.float32 and t.is_contiguous() and
-                            (n is None or t.numel() == n)),
-              f"{op}: inv_freq and norm weights must be contiguous float32, "
-              "norm weights [head_dim]")
-    if q is not None and q_out is None:
-        q_out = torch.empty((rows, n_heads, hd), dtype=q.dtype,
-                            device=q.device)
-    _need(q is None or (q_out.shape == q.shape and q_out.dtype == q.dtype and
-                        q_out.is_contiguous()),
-          f"{op}: q_out must be contiguous and match q")
-    for t in [q, k, v, q_out, *ints, *(t for t, _ in floats)]:
-        _need(t is None or t.device == store.device,
-              f"{op}: every tensor must be on the storage's device")
-    # (one row's stride is of no account: 0 rows apart)
-    stride = [0 if t is None else (t.stride(0) if rows > 1 else
-                                   t.shape[1] * hd) for t in (q, k, v)]
-    check(fn(store._pool, layer, _ptr(q), stride[0], _ptr(k), stride[1],
-             _ptr(v), stride[2], _DT[k.dtype], rows, n_heads, _ptr(q_norm),
-             _ptr(k_norm), float(eps), _ptr(positions) if rot else None,
-             _ptr(inv_freq), rot, int(bool(interleaved)), float(attn_factor),
-             _ptr(slot_block), _ptr(slot_off), _ptr(q_out)))
+        if (t.numel() != rows or t.dtype != torch.int32 or
+                not t.is_contiguous()):
+            raise RvkvError(f"{op}: positions/block_ids/offsets must be "
+                            "contiguous int32, one per row")
+    for t in (q_norm, k_norm):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.is_contiguous() and
+                  t.numel() == hd,
+                  f"{op}: norm weights must be contiguous float32 [head_dim]")
+            used.append(t)
+    _on(store, op, used)
+    check(fn(store._pool, layer, _ptr(q), qs, k.data_ptr(), ks, v.data_ptr(),
+             vs, _DT[dtype], rows, n_heads, _ptr(q_norm), _ptr(k_norm),
+             eps, _ptr(positions) if rot else None, _ptr(inv_freq), rot,
+             1 if interleaved else 0, attn_factor, slot_block.data_ptr(),
+             slot_off.data_ptr(), _ptr(q_out)))
     return q_out
 
 

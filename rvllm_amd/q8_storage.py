@@ -14,8 +14,9 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import check
-from .kv_storage import (_DT, HipGatherPlan, _need, _ptr, rope_append_call)
+from ._lib import RvkvError, check
+from .kv_storage import (_DT, HipGatherPlan, _need, _on, _ptr,
+                         rope_append_call)
 
 
 class HipQ8Storage:
@@ -54,6 +55,7 @@ class HipQ8Storage:
         if stream is None and self.device.type == "cuda":
             stream = torch.cuda.current_stream(self.device)
         self.stream = stream
+        self._views = {}  # (layer, which) -> codes, scales of this memory
         check(self._L.rvkv_q8_pool_create(
             n_layers, num_blocks, block_size, n_kv_heads, head_dim,
             _ptr(memory), memory.numel(),
@@ -85,27 +87,31 @@ class HipQ8Storage:
         n = self.n_kv_heads * self.block_size * (self.head_dim + 4)
         return -(-n // 256) * 256
 
+    def _view(self, layer: int, which: int):
+        got = self._views.get((layer, which))
+        if got is None:
+            _need(0 <= layer < self.n_layers and which in (0, 1),
+                  "q8: layer or which out of range")
+            rec, bs, hd = self._record(), self.block_size, self.head_dim
+            nb, kv = self.num_blocks, self.n_kv_heads
+            first = (2 * layer + which) * nb * rec
+            codes = self.memory.view(torch.int8).as_strided(
+                (nb, kv, bs, hd),
+                (rec, bs * hd) + ((hd, 1) if which == 0 else (1, bs)), first)
+            scales = self.memory[:self.nbytes].view(torch.float32).as_strided(
+                (nb, kv, bs), (rec // 4, bs, 1),
+                (first + kv * bs * hd) // 4)
+            got = self._views[layer, which] = codes, scales
+        return got
+
     def codes(self, layer: int, which: int) -> torch.Tensor:
         """int8 [num_blocks, n_kv, block_size, hd] of K (which 0) or V (1): a
         view, strided as the records lie (V's tokens are innermost)."""
-        _need(0 <= layer < self.n_layers and which in (0, 1),
-              "q8: layer or which out of range")
-        rec, bs, hd = self._record(), self.block_size, self.head_dim
-        return self.memory.view(torch.int8).as_strided(
-            (self.num_blocks, self.n_kv_heads, bs, hd),
-            (rec, bs * hd) + ((hd, 1) if which == 0 else (1, bs)),
-            (2 * layer + which) * self.num_blocks * rec)
+        return self._view(layer, which)[0]
 
     def scales(self, layer: int, which: int) -> torch.Tensor:
         """f32 [num_blocks, n_kv, block_size]: a view."""
-        _need(0 <= layer < self.n_layers and which in (0, 1),
-              "q8: layer or which out of range")
-        rec, bs, kv = self._record(), self.block_size, self.n_kv_heads
-        flat = self.memory[:self.nbytes].view(torch.float32)
-        return flat.as_strided(
-            (self.num_blocks, kv, bs), (rec // 4, bs, 1),
-            ((2 * layer + which) * self.num_blocks * rec
-             + kv * bs * self.head_dim) // 4)
+        return self._view(layer, which)[1]
 
     # -- append ---------------------------------------------------------------
     def rope_append(self, layer: int, q, k: torch.Tensor, v: torch.Tensor,
@@ -161,11 +167,10 @@ class HipQ8Storage:
         _need(out.shape == q.shape and out.dtype == q.dtype and
               out.is_contiguous(), f"{op}: out must match q")
         for t in ints:
-            _need(t.dtype == torch.int32 and t.is_contiguous(),
-                  f"{op}: index tensors must be contiguous int32")
-        for t in (q, out, *ints):
-            _need(t.device == self.device,
-                  f"{op}: every tensor must be on the storage's device")
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise RvkvError(f"{op}: index tensors must be contiguous "
+                                "int32")
+        _on(self, op, (q, out, *ints))
         return out
 
     def decode_workspace_bytes(self, batch: int, n_heads: int,
@@ -206,18 +211,25 @@ class HipQ8Storage:
             ws.numel() * ws.element_size()))
         return out
 
+    def prefill_workspace_bytes(self, rows: int, batch: int, n_heads: int,
+                                max_blocks: int, window: int = 0) -> int:
+        return self._L.rvkv_q8_prefill_workspace_bytes(
+            self._pool, rows, batch, n_heads, max_blocks, int(window or 0))
+
     def packed_prefill(self, layer: int, q: torch.Tensor,
                        row_start: torch.Tensor, block_tables: torch.Tensor,
                        pos_offset: torch.Tensor,
                        read_num_tokens: torch.Tensor,
                        out: Optional[torch.Tensor] = None,
+                       ws: Optional[torch.Tensor] = None,
                        scale: Optional[float] = None,
                        window: int = 0) -> torch.Tensor:
         """rvkv_q8_packed_prefill: causal attention of several sequences' query
         rows, packed. q [rows, n_heads, hd] f32 or f16; row_start [batch + 1],
         block_tables [batch, max_blocks], pos_offset and read_num_tokens
         [batch] u32. Rows of no sequence are left as they were in out (an out
-        made here holds anything there)."""
+        made here holds anything there). ws: scratch of
+        prefill_workspace_bytes(...), by default allocated here."""
         op = "packed_prefill"
         out = self._check_attn(op, q, out, (row_start, block_tables,
                                             pos_offset, read_num_tokens))
@@ -228,11 +240,17 @@ class HipQ8Storage:
         _need(pos_offset.numel() == batch and read_num_tokens.numel() == batch,
               f"{op}: pos_offset/read_num_tokens length must equal batch")
         rows, n_heads, hd = q.shape
+        wide, window = int(block_tables.shape[1]), int(window or 0)
         if scale is None:
             scale = 1.0 / math.sqrt(hd)
+        if ws is None:
+            need = self.prefill_workspace_bytes(rows, batch, n_heads, wide,
+                                                window)
+            if need:
+                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         check(self._L.rvkv_q8_packed_prefill(
             self._pool, layer, _ptr(q), _DT[q.dtype], _ptr(row_start), rows,
             _ptr(block_tables), _ptr(pos_offset), _ptr(read_num_tokens),
-            batch, block_tables.shape[1], n_heads, float(scale),
-            int(window or 0), _ptr(out)))
+            batch, wide, n_heads, float(scale), window, _ptr(out), _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size()))
         return out
