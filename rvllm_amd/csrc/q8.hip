@@ -1,5 +1,6 @@
 // q8.hip - the 8-bit paged cache's pool, its block copy and gather, and decode
 // attention over it.
+#include <cstdlib>
 #include <new>
 
 #include "q8.h"
@@ -40,6 +41,10 @@ size_t q8_bytes(const char *op, uint32_t n_layers, uint32_t num_blocks,
     fail(RVKV_EUNSUPPORTED, op,
          "block_size must be a multiple of 16; block_size and n_kv_heads at "
          "most 4096");
+    return 0;
+  }
+  if ((uint64_t)n_kv * block_size * (hd + 4) >> 31) {
+    fail(RVKV_EUNSUPPORTED, op, "a block's record must be below 2 GiB");
     return 0;
   }
   *rec = ((size_t)n_kv * block_size * (hd + 4) + 255) & ~(size_t)255;
@@ -110,13 +115,15 @@ __global__ void __launch_bounds__(256)
 //   s_j = scale ks_j (q . kcode_j),   out = sum_j p_j vs_j vcode_j / sum_j p_j,
 //   p_j = exp(s_j - max s), all keys j < ctx (and >= ctx - window).
 //
-// Both products run on v_mfma_f32_16x16x32_f16 with the keys, or the dims, as
-// the 16 rows and the heads of a KV group as the 16 columns: codes are exact
-// in f16, and the columns that a group of up to 8 heads leaves free carry the
-// f16 remainders of q and of the weights (column c the upper part of head c,
-// column c + 8 the lower), so q and the weights keep 21 bits or more and the
-// result is an f32 one at no extra product. Larger groups take n_sub
-// workgroups of up to 8 heads.
+// S = K q' on v_mfma_i32_16x16x64_i8: the codes as they lie in the cache, q as
+// a 24-bit fixed-point number relative to its head's largest value, in three
+// signed digits of base 256, each an operand of its own; integer sums are
+// exact. O = V' P on v_mfma_f32_16x16x32_f16: codes are exact in f16, the
+// weights two f16 parts. The 16 matrix rows are keys, or dims; the 16 columns
+// are the heads of a KV group, up to 8, twice: columns 0-7 the upper digit or
+// part, 8-15 the middle digit or lower part (the lowest digit takes a second
+// product). So an f32-accurate result costs no conversion of K and no product
+// more than a rounded one. Larger groups take n_sub workgroups.
 //
 // A wave takes 64 keys at a time and the workgroup's four waves take turns.
 // Row 4g + i of S tile t is key 16g + 4t + i, so lane group g of the result
@@ -132,7 +139,7 @@ struct DecodeArgs {
   float *ws_acc, *ws_ml;
   size_t rec;
   uint32_t n_heads, n_kv, group, n_sub, hd, bs, max_blocks, num_blocks;
-  uint32_t ctx_cap, part_tokens, n_parts;
+  uint32_t ctx_cap, part_tokens, n_parts, batch;
   float qscale;  // scale * log2(e)
   uint32_t window;
 };
@@ -155,12 +162,22 @@ __device__ __forceinline__ float ror8(float x) {
   return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x128,
                                                   0xf, 0xf, true));
 }
+// The largest of the four lanes of a column.
 __device__ __forceinline__ float max_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                                  __float_as_uint(x), false,
+                                                  false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(x),
+                                                  __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
 __device__ __forceinline__ half2v pk(float a, float b) {
   return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+__device__ __forceinline__ int4v load_nt(const unsigned char *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const int4v *>(p));
 }
 
 template <typename T, int HD>
@@ -170,8 +187,21 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   constexpr float kNone = -__builtin_inff();
   __shared__ float sh_acc[4][8][HD];
   __shared__ float sh_m[4][8], sh_l[4][8];
-  const uint32_t part = blockIdx.x, b = blockIdx.z;
-  const uint32_t kvh = blockIdx.y / a.n_sub, sub = blockIdx.y % a.n_sub;
+  // Workgroups: partitions outermost, so that those behind most sequences'
+  // ends do not share an XCD (workgroup id mod 8); the n_sub workgroups of a
+  // head, which read the same keys, eight apart, so that they do.
+  uint32_t unit, sub = 0;
+  if (a.n_sub == 1) {
+    unit = blockIdx.x;
+  } else {
+    const uint32_t eight = blockIdx.x / (8 * a.n_sub);
+    const uint32_t in = blockIdx.x - eight * 8 * a.n_sub;
+    sub = in / 8;
+    unit = eight * 8 + in % 8;
+  }
+  const uint32_t kvh = unit % a.n_kv, pb = unit / a.n_kv;
+  const uint32_t part = pb / a.batch, b = pb - part * a.batch;
+  if (part >= a.n_parts) return;  // (the last eight units may not be whole)
   const Range rg = visible(a, b);
   const uint64_t start64 = (uint64_t)rg.base + (uint64_t)part * a.part_tokens;
   if (a.n_parts > 1 && start64 >= rg.ctx) return;
@@ -184,38 +214,6 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   const bool has_head = h_in < a.group;
   const uint32_t head = kvh * a.group + (has_head ? h_in : 0);
   const uint32_t hd = a.hd, bs = a.bs, bsg = bs / 16;
-
-  // q of this lane's column: element u * 8 + j of chunk c is dim
-  // 64 c + 16 g + 8 u + j. Brought just below 2^15 by a power of two: neither
-  // part leaves f16's range, the lower one not its normal numbers.
-  half8v qf[NK][2];
-  float qscale = a.qscale;
-  {
-    const T *q = (const T *)a.q + ((size_t)b * a.n_heads + head) * hd;
-    float x[NK][16];
-    float top = 0.f;
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint32_t d = 64 * c + 16 * g + e;
-        x[c][e] = has_head && d < hd ? (float)q[d] : 0.f;
-        top = fmaxf(top, fabsf(x[c][e]));
-      }
-    top = max_groups(top);
-    const uint32_t ex = scale_exponent(top);
-    const float down = __uint_as_float((269 - ex) << 23);
-    qscale *= __uint_as_float((ex - 15) << 23);
-    const float part_of = col >= 8 ? 1.f : 0.f;
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float y = x[c][e] * down;
-        qf[c][e >> 3][e & 7] =
-            (_Float16)__builtin_fmaf(-part_of, (float)(_Float16)y, y);
-      }
-  }
 
   const uint32_t n_tiles = end > start ? (end - start + 63) / 64 : 0;
   const uint32_t last_granule = rg.ctx ? (rg.ctx - 1) / 16 : 0;
@@ -234,26 +232,26 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     p.blk = table[bi];
     return p;
   };
-  uint4 kr[4 * NK], vr[NV];
+  int4v kr[4 * NK], vr[NV];
   float ks[16], vs[16];
-  bool seen;  // this lane group's keys lie in a readable block
+  bool seen = false;  // this lane group's keys lie in a readable block
   const uint32_t gk = col >> 2;
+  const uint32_t k_at = kvh * bs * hd + (col & 3) * hd + g * 16;
+  const uint32_t v_at = kvh * bs * hd + col * bs;
+  const uint32_t s_at = a.n_kv * hd * bs + kvh * bs * 4;
   const auto load_k = [&](Place p) {
     const uint32_t blk = p.blk < a.num_blocks ? p.blk : 0;
-    const unsigned char *kp = a.kc + blk * a.rec + (size_t)kvh * bs * hd +
-                              (p.in * 16 + (col & 3)) * hd + g * 16;
+    const unsigned char *kp = a.kc + blk * a.rec + (k_at + p.in * 16 * hd);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int c = 0; c < NK; ++c)
-        kr[t * NK + c] = *reinterpret_cast<const uint4 *>(
-            kp + t * 4 * hd + (c * 64 + g * 16 < hd ? c * 64 : 0));
+        kr[t * NK + c] = load_nt(
+            kp + t * 4 * hd + ((uint32_t)c * 64 + g * 16 < hd ? c * 64 : 0));
   };
   const auto load_scales = [&](Place p) {
     seen = p.blk < a.num_blocks;
-    const uint32_t blk = seen ? p.blk : 0;
-    const size_t at = blk * a.rec + (size_t)a.n_kv * bs * hd +
-                      ((size_t)kvh * bs + p.in * 16) * 4;
+    const size_t at = (seen ? p.blk : 0) * a.rec + (s_at + p.in * 64);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       *reinterpret_cast<float4 *>(ks + 4 * i) =
@@ -264,16 +262,16 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   };
   const auto load_v = [&](Place p) {
     const uint32_t blk = p.blk < a.num_blocks ? p.blk : 0;
-    const unsigned char *vp = a.vc + blk * a.rec + (size_t)kvh * bs * hd +
-                              col * bs + p.in * 16;
+    const unsigned char *vp = a.vc + blk * a.rec + (v_at + p.in * 16);
 #pragma unroll
-    for (int d = 0; d < NV; ++d)
-      if ((uint32_t)d * 16 < hd)
-        vr[d] = *reinterpret_cast<const uint4 *>(vp + d * 16 * bs);
+    for (int d = 0; d < NV; ++d)  // (rows from hd on: any codes, not stored)
+      vr[d] = load_nt(vp + ((uint32_t)d * 16 < hd ? d * 16 * bs : 0));
   };
 
   float m = kNone, l = 0.f;
-  float vnorm = kVnorm0;  // power of two above every vs
+  // Weights are held as 2^shift p, l with them: times vs, they stay below 2^15,
+  // and their lower parts in f16's normal numbers.
+  int shift = 95;
   float4v acc[NV];
 #pragma unroll
   for (int d = 0; d < NV; ++d) acc[d] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -285,32 +283,92 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     load_k(pk0);
     load_scales(pv0);
     load_v(pv0);
+
+    // q's digits: byte e of chunk c is dim 64 c + 16 g + e of this column's
+    // head. A digit is in -128 .. 127, so q's largest value is brought below
+    // 127/128 of 2^23.
+    int4v qd[NK], q0[NK];
+    // qscale: |scale| log2(e) / q's power of two; the sign goes with q.
+    float qscale = fmaxf(fabsf(a.qscale), 0x1p-100f);
+    {
+      const T *q = (const T *)a.q + ((size_t)b * a.n_heads + head) * hd;
+      float x[NK][16];
+      float top = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; e += 16 / (int)sizeof(T)) {
+          const uint32_t d = 64 * c + 16 * g + e;
+          alignas(16) T y[16 / sizeof(T)];
+          *reinterpret_cast<uint4 *>(y) = uint4{};
+          if (has_head && 64 * c + 16 * g < hd)
+            *reinterpret_cast<uint4 *>(y) =
+                *reinterpret_cast<const uint4 *>(q + d);
+#pragma unroll
+          for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+            x[c][e + i] = (float)y[i];
+            const float mag = fabsf(x[c][e + i]);
+            finite = finite && mag < __builtin_inff();
+            top = fmaxf(top, mag);
+          }
+        }
+      top = max_groups(top);
+      uint32_t ex = scale_exponent(top);  // top < 2^(ex - 127)
+      ex = ex < 64 ? 64 : ex;
+      float up = __uint_as_float((277 - ex) << 23) * (127.f / 128.f);
+      if (a.qscale < 0.f) up = -up;
+      qscale *= __uint_as_float((ex - 23) << 23) * (128.f / 127.f);
+      // (a head whose q is not finite: every score, and so its row, is NaN)
+      if (max_groups(finite ? 0.f : 1.f) > 0.f) qscale = __builtin_nanf("");
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t mine = 0, low = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int v = (int)__builtin_rintf(x[c][4 * w + i] * up);
+            const int d0 = (int)(signed char)v, v1 = (v - d0) >> 8;
+            const int d1 = (int)(signed char)v1, d2 = (v1 - d1) >> 8;
+            mine |= (uint32_t)((col < 8 ? d2 : d1) & 255) << (8 * i);
+            low |= (uint32_t)((col < 8 ? d0 : 0) & 255) << (8 * i);
+          }
+          qd[c][w] = (int)mine;
+          q0[c][w] = (int)low;
+        }
+    }
+    const float digit = col < 8 ? 65536.f : 256.f;
+
     for (uint32_t tile = wave; tile < n_tiles; tile += 4) {
       const bool more = tile + 4 < n_tiles;
       float s[16];
+      float top = kNone;
       {
-        float4v st[4];
+        int4v st[4], s0[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          st[t] = float4v{0.f, 0.f, 0.f, 0.f};
+          st[t] = s0[t] = int4v{0, 0, 0, 0};
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
-            const uint4 k = kr[t * NK + c];
-            st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                codes_to_half8(k.x, k.y), qf[c][0], st[t], 0, 0, 0);
-            st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                codes_to_half8(k.z, k.w), qf[c][1], st[t], 0, 0, 0);
+            st[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                kr[t * NK + c], qd[c], st[t], 0, 0, 0);
+            s0[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                kr[t * NK + c], q0[c], s0[t], 0, 0, 0);
           }
         }
+        if (more) load_k(pk1);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = st[j >> 2][j & 3];
+        for (int j = 0; j < 16; ++j) {
+          const float x = __builtin_fmaf((float)st[j >> 2][j & 3], digit,
+                                         (float)s0[j >> 2][j & 3]);
+          s[j] = (x + ror8(x)) * ks[j];
+        }
       }
-      if (more) load_k(pk1);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = (s[j] + ror8(s[j])) * (ks[j] * qscale);
       const uint32_t key = start + tile * 64 + 16 * g;
       if (start + tile * 64 < rg.lo || start + tile * 64 + 64 > end ||
           !__all(seen)) {
+        asm volatile("");  // (a branch, no selects on every tile)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const bool ok = seen && key + j >= rg.lo && key + j < end;
@@ -318,38 +376,37 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
           vs[j] = ok ? vs[j] : 0.f;
         }
       }
-      float top = s[0], vtop = vs[0];
+      float vtop = 0.f;
 #pragma unroll
-      for (int j = 1; j < 16; ++j) {
-        top = fmaxf(top, s[j]);
-        vtop = fmaxf(vtop, vs[j]);
+      for (int j = 0; j < 16; j += 2) {
+        top = fmaxf(fmaxf(s[j], s[j + 1]), top);
+        vtop = fmaxf(fmaxf(vs[j], vs[j + 1]), vtop);
       }
-      const float m_new = fmaxf(m, max_groups(top));
+      top *= qscale;
+      top = max_groups(top);
       vtop = max_groups(vtop);
-      const float mm = m_new == kNone ? 0.f : m_new;
-      float fix = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-      if (m == m_new) fix = 1.f;
-      m = m_new;
-      l *= fix;
-      if (vtop >= vnorm) {  // (uniform over the wave)
-        uint32_t e = (__float_as_uint(vtop) >> 23) + 1;
-        e = e > 253 ? 253 : e;
-        const float now = __uint_as_float(e << 23);
-        fix *= vnorm / now;
-        vnorm = now;
-      }
-      if (!__all(fix == 1.f)) {
+      if (__any(top > m) || vtop >= __uint_as_float((uint32_t)(142 - shift)
+                                                    << 23)) {
+        asm volatile("");
+        const float now = fmaxf(m, top);
+        float fix = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        // vs < 2^(15 - shift)
+        const int e = (int)(__float_as_uint(vtop) >> 23) - 126;
+        const int to = 15 - e < shift ? 15 - e : shift;
+        fix = __builtin_amdgcn_ldexpf(fix, to - shift);
+        shift = to;
+        l *= fix;
 #pragma unroll
         for (int d = 0; d < NV; ++d) acc[d] *= fix;
       }
-      // (weights up to 2^15, as q)
-      const float vdown =
-          __uint_as_float((269u << 23) - __float_as_uint(vnorm));
+      const float mm = (m == kNone ? 0.f : m) - (float)shift;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float p = __builtin_amdgcn_exp2f(s[j] - mm);
+        const float p =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], qscale, -mm));
         l += p;
-        s[j] = p * (vs[j] * vdown);
+        s[j] = p * vs[j];
       }
       if (more) load_scales(pv1);
       half8v pf[2];
@@ -366,12 +423,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
         }
 #pragma unroll
       for (int d = 0; d < NV; ++d) {
-        if ((uint32_t)d * 16 < hd) {
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              codes_to_half8(vr[d].x, vr[d].y), pf[0], acc[d], 0, 0, 0);
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              codes_to_half8(vr[d].z, vr[d].w), pf[1], acc[d], 0, 0, 0);
-        }
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            codes_to_half8(vr[d][0], vr[d][1]), pf[0], acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            codes_to_half8(vr[d][2], vr[d][3]), pf[1], acc[d], 0, 0, 0);
       }
       if (more) {
         load_v(pv1);
@@ -384,15 +439,16 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   }
 
   // Merge the waves: a head's weights relative to the largest maximum.
+  const float back = __builtin_amdgcn_ldexpf(1.f, -shift);
   if (lane < 8) {
     sh_m[wave][lane] = m;
-    sh_l[wave][lane] = l;
+    sh_l[wave][lane] = l * back;
   }
 #pragma unroll
   for (int d = 0; d < NV; ++d) {
     float4v o = acc[d];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (o[i] + ror8(o[i])) * (vnorm * 0x1p-15f);
+    for (int i = 0; i < 4; ++i) o[i] = (o[i] + ror8(o[i])) * back;
     if (col < 8)
       *reinterpret_cast<float4v *>(&sh_acc[wave][col][d * 16 + 4 * g]) = o;
   }
@@ -406,7 +462,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     float o = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = sh_m[w][h] == kNone ? 0.f : __builtin_amdgcn_exp2f(sh_m[w][h] - top);
+      const float f = sh_m[w][h] == kNone
+                          ? 0.f : __builtin_amdgcn_exp2f(sh_m[w][h] - top);
       o += sh_acc[w][h][d] * f;
       sum += sh_l[w][h] * f;
     }
@@ -460,6 +517,13 @@ __global__ void __launch_bounds__(256) q8_reduce_kernel(DecodeArgs a) {
   }
 }
 
+// Workgroups of a decode launch.
+uint64_t decode_groups(uint64_t n_parts, uint32_t batch, uint32_t n_kv,
+                       uint32_t n_sub) {
+  const uint64_t units = n_parts * batch * n_kv;
+  return n_sub == 1 ? units : (units + 7) / 8 * 8 * n_sub;
+}
+
 uint32_t hd_up(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Keys of a partition, a multiple of 256 (64 for each of the four waves).
@@ -469,7 +533,9 @@ uint32_t partition_tokens(const rvkv_q8_pool *p, uint32_t batch,
   const uint64_t rows = (uint64_t)batch * p->n_kv * n_sub;
   const uint64_t want = ((uint64_t)keys * rows + 1023) / 1024;
   uint64_t t = (want + 255) / 256 * 256;
-  return (uint32_t)(t < 256 ? 256 : t > 1024 ? 1024 : t);
+  const char *e1 = getenv("PMAX");
+  uint64_t mx = e1 ? atoi(e1) : 1024;
+  return (uint32_t)(t < 256 ? 256 : t > mx ? mx : t);
 }
 
 struct Layout {
@@ -495,8 +561,9 @@ template <typename T, int HD>
 int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
                   hipStream_t st) {
   hipLaunchKernelGGL((q8_decode_kernel<T, HD>),
-                     dim3(a.n_parts, a.n_kv * a.n_sub, batch), dim3(256), 0, st,
-                     a);
+                     dim3((uint32_t)decode_groups(a.n_parts, batch, a.n_kv,
+                                                  a.n_sub)),
+                     dim3(256), 0, st, a);
   if (a.n_parts > 1)
     hipLaunchKernelGGL((q8_reduce_kernel<T, HD>), dim3(a.n_heads, batch),
                        dim3(256), 0, st, a);
@@ -538,7 +605,8 @@ int rvkv_q8_pool_create(uint32_t n_layers, uint32_t num_blocks,
                                 n_kv_heads, head_dim, &rec);
   if (!bytes)
     return head_dim % 16 || head_dim > 256 || block_size % 16 ||
-                   block_size > 4096 || n_kv_heads > 4096
+                   block_size > 4096 || n_kv_heads > 4096 ||
+                   (uint64_t)n_kv_heads * block_size * (head_dim + 4) >> 31
                ? RVKV_EUNSUPPORTED : RVKV_EINVAL;
   if (memory && memory_bytes < bytes)
     return fail(RVKV_EINVAL, op, "memory smaller than the required bytes");
@@ -697,13 +765,16 @@ int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
   if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
     return fail(RVKV_EINVAL, op, "q and out must be 16-byte aligned");
   const uint32_t group = n_heads / pool->n_kv, n_sub = (group + 7) / 8;
-  if ((uint64_t)pool->n_kv * n_sub > 65535)
+  if (n_heads > 65535)
     return fail(RVKV_EUNSUPPORTED, op, "head count too large");
   const uint64_t cap = (uint64_t)max_blocks * pool->block_size;
   if (max_ctx_len == 0) max_ctx_len = 1;
   if (max_ctx_len > rvkv_detail::kMaxKeys) max_ctx_len = rvkv_detail::kMaxKeys;
   const Layout w = layout(pool, batch, n_heads, max_ctx_len,
                           window > 0 ? (uint32_t)window : 0);
+  // (a launch holds fewer than 2^32 threads)
+  if (decode_groups(w.n_parts, batch, pool->n_kv, n_sub) > 0xffffffu)
+    return fail(RVKV_EUNSUPPORTED, op, "too many partitions for one launch");
   if (w.bytes) {
     if (!ws) return fail(RVKV_EINVAL, op, "workspace is NULL");
     if (ws_bytes < w.bytes)
@@ -734,6 +805,7 @@ int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
   a.ctx_cap = (uint32_t)(cap < max_ctx_len ? cap : max_ctx_len);
   a.part_tokens = w.part_tokens;
   a.n_parts = w.n_parts;
+  a.batch = batch;
   a.qscale = scale * kLog2e;
   a.window = window > 0 ? (uint32_t)window : 0;
   return dtype == RVKV_F16 ? launch_decode<_Float16>(op, a, batch, pool->stream)

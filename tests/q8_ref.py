@@ -50,10 +50,12 @@ def attend(q, k, v, seen, scale):
     """q [rows, H, hd], k, v [keys, kv, hd], seen [rows, keys]; f64. Returns
     the result and a bound of what an f32-accurate kernel may be off by.
 
-    With u = 2^-24, per (row, head): q is held to 2^-23 of its largest value
-    (two f16 parts) and a score's hd + 4 products and sums round by u each, so
-    a score is off by at most ds = scale (2u max|q| sum|k| + (hd + 4) u
-    sum|q k|) and a weight by ds relative to it, in the sum and in the
+    With u = 2^-24, per (row, head): q is held as two f16 parts, to 2u of its
+    largest value, or as a fixed-point number below 127/128 2^23: off by half a
+    unit and by u of itself, half a unit again, and the largest value is above
+    127/128 2^22 units, so to 1 / (127/128 2^22) < 5u of it. A score's hd + 4
+    products and sums round by u each, so it is off by at most ds = scale (5u
+    max|q| sum|k| + (hd + 4) u sum|q k|) and a weight by ds relative to it, in the sum and in the
     products. A weight is cut to two f16 parts of 10 bits and more: 2^-20 = 16u
     of itself, or the smallest f16 step, 2u of the largest value. Sums over m
     keys round by m u, twice. With the largest weight 1, the weights' sum l is
@@ -76,7 +78,7 @@ def attend(q, k, v, seen, scale):
         l = w.sum(-1, keepdim=True)
         out[:, h] = torch.where(l > 0, (w @ vh) / l.clamp(min=1e-300), 0.0)
         ka = kh.abs()
-        ds = scale * (2 * u * qh.abs().amax(-1, keepdim=True) * ka.sum(-1)
+        ds = scale * (5 * u * qh.abs().amax(-1, keepdim=True) * ka.sum(-1)
                       + (hd + 4) * u * (qh.abs() @ ka.T))
         ds = torch.where(seen, ds, 0.0).amax(-1)
         vmax = torch.where(seen, vh.abs().amax(-1)[None], 0.0).amax(-1)
