@@ -42,6 +42,11 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
+// A value that is the wave's, as the compiler cannot tell by itself.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
 // Four int8 codes as f16, exactly: code ^ 0x80 = code + 128 in a byte below
 // 0x64 is the f16 1024 + 128 + code; one subtraction leaves the code.
 __device__ __forceinline__ void codes_to_half4(uint32_t c, half2v &lo,

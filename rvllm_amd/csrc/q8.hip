@@ -1,7 +1,7 @@
 // q8.hip - the 8-bit paged cache's pool, its block copy and gather, and decode
 // attention over it.
-#include <cstdlib>
 #include <new>
+#include <type_traits>
 
 #include "q8.h"
 
@@ -173,6 +173,18 @@ __device__ __forceinline__ float max_groups(float x) {
                                                   false);
   return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
+// The largest of a wave.
+__device__ __forceinline__ float max_wave(float x) {
+  const auto dpp = [](float v, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(
+        __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x121>()));  // row_ror 1
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x122>()));  // 2
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x124>()));  // 4
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x128>()));  // 8
+  return max_groups(x);
+}
 __device__ __forceinline__ half2v pk(float a, float b) {
   return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
@@ -180,13 +192,15 @@ __device__ __forceinline__ int4v load_nt(const unsigned char *p) {
   return __builtin_nontemporal_load(reinterpret_cast<const int4v *>(p));
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
+template <typename T, int HD, int W>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2)
     q8_decode_kernel(DecodeArgs a) {
   constexpr int NK = HD / 64, NV = HD / 16;
   constexpr float kNone = -__builtin_inff();
-  __shared__ float sh_acc[4][8][HD];
-  __shared__ float sh_m[4][8], sh_l[4][8];
+  __shared__ float sh_acc[W][8][HD];
+  __shared__ float sh_m[W][8], sh_l[W][8];
+  // A tile's scales, from one key a lane to the 16 of a lane group.
+  __shared__ __align__(16) float sh_ks[W][64], sh_vs[W][64];
   // Workgroups: partitions outermost, so that those behind most sequences'
   // ends do not share an XCD (workgroup id mod 8); the n_sub workgroups of a
   // head, which read the same keys, eight apart, so that they do.
@@ -208,7 +222,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   const uint32_t start = (uint32_t)start64;
   const uint32_t end = rg.ctx - start < a.part_tokens ? rg.ctx
                                                       : start + a.part_tokens;
-  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const uint32_t col = lane & 15, g = lane >> 4;
   const uint32_t h_in = sub * 8 + (col & 7);
   const bool has_head = h_in < a.group;
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     return p;
   };
   int4v kr[4 * NK], vr[NV];
-  float ks[16], vs[16];
+  float ks1, vs1;     // of key lane of the tile
   bool seen = false;  // this lane group's keys lie in a readable block
   const uint32_t gk = col >> 2;
   const uint32_t k_at = kvh * bs * hd + (col & 3) * hd + g * 16;
@@ -251,14 +265,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   };
   const auto load_scales = [&](Place p) {
     seen = p.blk < a.num_blocks;
-    const size_t at = (seen ? p.blk : 0) * a.rec + (s_at + p.in * 64);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<float4 *>(ks + 4 * i) =
-          *reinterpret_cast<const float4 *>(a.kc + at + 16 * i);
-      *reinterpret_cast<float4 *>(vs + 4 * i) =
-          *reinterpret_cast<const float4 *>(a.vc + at + 16 * i);
-    }
+    const size_t at = (seen ? p.blk : 0) * a.rec + (s_at + p.in * 64 + col * 4);
+    ks1 = *reinterpret_cast<const float *>(a.kc + at);
+    vs1 = *reinterpret_cast<const float *>(a.vc + at);
   };
   const auto load_v = [&](Place p) {
     const uint32_t blk = p.blk < a.num_blocks ? p.blk : 0;
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
 
   if (wave < n_tiles) {
     Place pk0 = place(wave, gk), pv0 = place(wave, g);
-    Place pk1 = place(wave + 4, gk), pv1 = place(wave + 4, g);
+    Place pk1 = place(wave + W, gk), pv1 = place(wave + W, g);
     load_k(pk0);
     load_scales(pv0);
     load_v(pv0);
@@ -340,51 +349,52 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     }
     const float digit = col < 8 ? 65536.f : 256.f;
 
-    for (uint32_t tile = wave; tile < n_tiles; tile += 4) {
-      const bool more = tile + 4 < n_tiles;
+    for (uint32_t tile = wave; tile < n_tiles; tile += W) {
+      const bool more = tile + W < n_tiles;
+      const uint32_t first = start + tile * 64;
+      const bool masked = first < rg.lo || first + 64 > end || !__all(seen);
+      bool ok = true;
+      if (masked) {
+        const uint32_t key = first + lane;
+        ok = seen && key >= rg.lo && key < end;
+        if (!ok) ks1 = vs1 = 0.f;
+      }
+      const uint64_t keep = __ballot(ok) >> (16 * g);
+      sh_ks[wave][lane] = ks1;
+      sh_vs[wave][lane] = vs1;
+      __builtin_amdgcn_wave_barrier();
+      float vtop = vs1;
       float s[16];
       float top = kNone;
-      {
-        int4v st[4], s0[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          st[t] = s0[t] = int4v{0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) {
+        int4v st = {0, 0, 0, 0}, s0 = {0, 0, 0, 0};
 #pragma unroll
-          for (int c = 0; c < NK; ++c) {
-            st[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                kr[t * NK + c], qd[c], st[t], 0, 0, 0);
-            s0[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                kr[t * NK + c], q0[c], s0[t], 0, 0, 0);
-          }
+        for (int c = 0; c < NK; ++c) {
+          st = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t * NK + c], qd[c], st,
+                                                     0, 0, 0);
+          s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t * NK + c], q0[c], s0,
+                                                     0, 0, 0);
         }
-        if (more) load_k(pk1);
+        const float4v ks = *reinterpret_cast<const float4v *>(
+            &sh_ks[wave][16 * g + 4 * t]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float x = __builtin_fmaf((float)st[j >> 2][j & 3], digit,
-                                         (float)s0[j >> 2][j & 3]);
-          s[j] = (x + ror8(x)) * ks[j];
+        for (int i = 0; i < 4; ++i) {
+          const float x = __builtin_fmaf((float)st[i], digit, (float)s0[i]);
+          s[4 * t + i] = (x + ror8(x)) * ks[i];
         }
       }
-      const uint32_t key = start + tile * 64 + 16 * g;
-      if (start + tile * 64 < rg.lo || start + tile * 64 + 64 > end ||
-          !__all(seen)) {
+      if (more) load_k(pk1);
+      if (masked) {
         asm volatile("");  // (a branch, no selects on every tile)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const bool ok = seen && key + j >= rg.lo && key + j < end;
-          s[j] = ok ? s[j] : kNone;
-          vs[j] = ok ? vs[j] : 0.f;
-        }
+        for (int j = 0; j < 16; ++j) s[j] = keep >> j & 1 ? s[j] : kNone;
       }
-      float vtop = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        top = fmaxf(fmaxf(s[j], s[j + 1]), top);
-        vtop = fmaxf(fmaxf(vs[j], vs[j + 1]), vtop);
-      }
+      for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(s[j], s[j + 1]), top);
       top *= qscale;
       top = max_groups(top);
-      vtop = max_groups(vtop);
+      vtop = max_wave(vtop);
       if (__any(top > m) || vtop >= __uint_as_float((uint32_t)(142 - shift)
                                                     << 23)) {
         asm volatile("");
@@ -402,12 +412,18 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
       }
       const float mm = (m == kNone ? 0.f : m) - (float)shift;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float p =
-            __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], qscale, -mm));
-        l += p;
-        s[j] = p * vs[j];
+      for (int t = 0; t < 4; ++t) {
+        const float4v vs = *reinterpret_cast<const float4v *>(
+            &sh_vs[wave][16 * g + 4 * t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(s[4 * t + i], qscale, -mm));
+          l += p;
+          s[4 * t + i] = p * vs[i];
+        }
       }
+      __builtin_amdgcn_wave_barrier();
       if (more) load_scales(pv1);
       half8v pf[2];
 #pragma unroll
@@ -430,8 +446,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
       }
       if (more) {
         load_v(pv1);
-        pk1 = place(tile + 8, gk);
-        pv1 = place(tile + 8, g);
+        pk1 = place(tile + 2 * W, gk);
+        pv1 = place(tile + 2 * W, g);
       }
     }
     l += __shfl_xor(l, 16);
@@ -453,15 +469,15 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
       *reinterpret_cast<float4v *>(&sh_acc[wave][col][d * 16 + 4 * g]) = o;
   }
   __syncthreads();
-  for (uint32_t x = threadIdx.x; x < 8 * HD; x += 256) {
+  for (uint32_t x = threadIdx.x; x < 8 * HD; x += 64 * W) {
     const uint32_t h = x / HD, d = x % HD;
     if (sub * 8 + h >= a.group || d >= hd) continue;
     float top = sh_m[0][h];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sh_m[w][h]);
+    for (int w = 1; w < W; ++w) top = fmaxf(top, sh_m[w][h]);
     float o = 0.f, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = sh_m[w][h] == kNone
                           ? 0.f : __builtin_amdgcn_exp2f(sh_m[w][h] - top);
       o += sh_acc[w][h][d] * f;
@@ -481,39 +497,62 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   }
 }
 
-// Merges a head's partitions: 256 threads, 256 / HD partitions at a time.
+// Merges a head's partitions: every partition's weight into LDS, then
+// 1024 / HD partitions at a time, four dims a thread.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) q8_reduce_kernel(DecodeArgs a) {
-  constexpr int W = 256 / HD;
+  constexpr uint32_t D4 = HD / 4, P = 256 / D4;
   constexpr float kNone = -__builtin_inff();
-  __shared__ float sh_o[256], sh_l[W];
-  const uint32_t h = blockIdx.x, b = blockIdx.y;
+  __shared__ float weight[256], sh_top[4], sh_sum[4];
+  __shared__ __align__(16) float sh_o[P][HD];
+  const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const Range rg = visible(a, b);
   const uint32_t live =
       rg.ctx > rg.base
           ? (rg.ctx - rg.base + a.part_tokens - 1) / a.part_tokens : 0;
   const size_t row = (size_t)b * a.n_heads + h;
-  const float *ml = a.ws_ml + row * a.n_parts * 2;
+  const float2 *ml =
+      reinterpret_cast<const float2 *>(a.ws_ml) + row * a.n_parts;
   const float *acc = a.ws_acc + row * a.n_parts * HD;
-  const uint32_t d = threadIdx.x % HD, w = threadIdx.x / HD;
+  const uint32_t d = tid % D4 * 4, w = tid / D4;
+  // The largest maximum (most calls have at most 256 partitions: one load).
+  float2 mine = {kNone, 0.f};
   float top = kNone;
-  for (uint32_t p = 0; p < live; ++p) top = fmaxf(top, ml[2 * p]);
-  float o = 0.f, sum = 0.f;
-  for (uint32_t p = w; p < live; p += W) {
-    const float f = ml[2 * p] == kNone ? 0.f : __builtin_amdgcn_exp2f(ml[2 * p] - top);
-    sum += ml[2 * p + 1] * f;
-    if (d < a.hd) o += acc[(size_t)p * HD + d] * f;
+  for (uint32_t p = tid; p < live; p += 256) {
+    mine = ml[p];
+    top = fmaxf(top, mine.x);
   }
-  sh_o[threadIdx.x] = o;
-  if (d == 0) sh_l[w] = sum;
+  top = max_wave(top);
+  if ((tid & 63) == 0) sh_top[tid >> 6] = top;
   __syncthreads();
-  if (w == 0 && d < a.hd) {
+  top = fmaxf(fmaxf(sh_top[0], sh_top[1]), fmaxf(sh_top[2], sh_top[3]));
+  float4v o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (uint32_t p0 = 0; p0 < live; p0 += 256) {
+    const uint32_t n = live - p0 < 256 ? live - p0 : 256;
+    if (live > 256) mine = tid < n ? ml[p0 + tid] : float2{kNone, 0.f};
+    const float f =
+        mine.x == kNone ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
+    sum += mine.y * f;
+    weight[tid] = f;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t p = w; p < n; p += P)
+      o += *reinterpret_cast<const float4v *>(acc + (size_t)(p0 + p) * HD + d) *
+           weight[p];
+    __syncthreads();
+  }
 #pragma unroll
-    for (int i = 1; i < W; ++i) {
-      o += sh_o[i * HD + d];
-      sum += sh_l[i];
-    }
-    ((T *)a.out)[row * a.hd + d] = (T)(sum == 0.f ? 0.f : o / sum);
+  for (int i = 32; i >= 1; i >>= 1) sum += __shfl_xor(sum, i);
+  if ((tid & 63) == 0) sh_sum[tid >> 6] = sum;
+  *reinterpret_cast<float4v *>(&sh_o[w][d]) = o;
+  __syncthreads();
+  sum = sh_sum[0] + sh_sum[1] + sh_sum[2] + sh_sum[3];
+  if (tid < a.hd) {
+    float x = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < P; ++i) x += sh_o[i][tid];
+    ((T *)a.out)[row * a.hd + tid] = (T)(sum == 0.f ? 0.f : x / sum);
   }
 }
 
@@ -526,20 +565,29 @@ uint64_t decode_groups(uint64_t n_parts, uint32_t batch, uint32_t n_kv,
 
 uint32_t hd_up(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Keys of a partition, a multiple of 256 (64 for each of the four waves).
-uint32_t partition_tokens(const rvkv_q8_pool *p, uint32_t batch,
-                          uint32_t n_heads, uint32_t keys) {
+// How a launch is cut. waves 4: a workgroup's waves take a partition's tiles
+// in turn; partitions of 256 to 2048 keys, so that up to 512 workgroups (two
+// a CU) share the keys (2 x 32749 keys of 8 heads: 1024-key partitions 31 us,
+// 512 36, 256 43; 64 x 2048: 2048 34 us, 1024 39). waves 1: launches with
+// 1024-key partitions for 4096 waves or more, where single waves balance
+// ragged contexts better and need no merge in the workgroup (300 contexts up
+// to 8192 of 8 heads: 190 us; four waves 218, at 2048 keys 206; 256 x 4096
+// 370, four waves 415 and 377).
+struct Cut {
+  uint32_t part_tokens, waves;
+};
+Cut cut(const rvkv_q8_pool *p, uint32_t batch, uint32_t n_heads,
+        uint32_t keys) {
   const uint32_t n_sub = (n_heads / p->n_kv + 7) / 8;
   const uint64_t rows = (uint64_t)batch * p->n_kv * n_sub;
-  const uint64_t want = ((uint64_t)keys * rows + 1023) / 1024;
-  uint64_t t = (want + 255) / 256 * 256;
-  const char *e1 = getenv("PMAX");
-  uint64_t mx = e1 ? atoi(e1) : 1024;
-  return (uint32_t)(t < 256 ? 256 : t > mx ? mx : t);
+  if (rows * (((uint64_t)keys + 1023) / 1024) >= 4096) return {1024, 1};
+  const uint64_t want = ((uint64_t)keys * rows + 511) / 512;
+  const uint64_t t = (want + 255) / 256 * 256;
+  return {(uint32_t)(t < 256 ? 256 : t > 2048 ? 2048 : t), 4};
 }
 
 struct Layout {
-  uint32_t part_tokens, n_parts;
+  uint32_t part_tokens, n_parts, waves;
   size_t ml_off, bytes;
 };
 // window 0: none. A window's first partition starts up to 15 keys before it.
@@ -548,7 +596,9 @@ Layout layout(const rvkv_q8_pool *p, uint32_t batch, uint32_t n_heads,
   Layout w{};
   uint64_t keys = max_ctx ? max_ctx : 1;
   if (window && (uint64_t)window + 15 < keys) keys = (uint64_t)window + 15;
-  w.part_tokens = partition_tokens(p, batch, n_heads, (uint32_t)keys);
+  const Cut c = cut(p, batch, n_heads, (uint32_t)keys);
+  w.part_tokens = c.part_tokens;
+  w.waves = c.waves;
   w.n_parts = (uint32_t)((keys + w.part_tokens - 1) / w.part_tokens);
   if (w.n_parts <= 1) return w;
   const size_t slots = (size_t)batch * n_heads * w.n_parts;
@@ -559,11 +609,12 @@ Layout layout(const rvkv_q8_pool *p, uint32_t batch, uint32_t n_heads,
 
 template <typename T, int HD>
 int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
-                  hipStream_t st) {
-  hipLaunchKernelGGL((q8_decode_kernel<T, HD>),
-                     dim3((uint32_t)decode_groups(a.n_parts, batch, a.n_kv,
-                                                  a.n_sub)),
-                     dim3(256), 0, st, a);
+                  uint32_t waves, hipStream_t st) {
+  const dim3 grid((uint32_t)decode_groups(a.n_parts, batch, a.n_kv, a.n_sub));
+  if (waves == 4)
+    hipLaunchKernelGGL((q8_decode_kernel<T, HD, 4>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((q8_decode_kernel<T, HD, 1>), grid, dim3(64), 0, st, a);
   if (a.n_parts > 1)
     hipLaunchKernelGGL((q8_reduce_kernel<T, HD>), dim3(a.n_heads, batch),
                        dim3(256), 0, st, a);
@@ -573,11 +624,11 @@ int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
 
 template <typename T>
 int launch_decode(const char *op, const DecodeArgs &a, uint32_t batch,
-                  hipStream_t st) {
+                  uint32_t waves, hipStream_t st) {
   switch (hd_up(a.hd)) {
-    case 64: return launch_decode<T, 64>(op, a, batch, st);
-    case 128: return launch_decode<T, 128>(op, a, batch, st);
-    default: return launch_decode<T, 256>(op, a, batch, st);
+    case 64: return launch_decode<T, 64>(op, a, batch, waves, st);
+    case 128: return launch_decode<T, 128>(op, a, batch, waves, st);
+    default: return launch_decode<T, 256>(op, a, batch, waves, st);
   }
 }
 
@@ -808,8 +859,9 @@ int rvkv_q8_paged_decode(const rvkv_q8_pool *pool, uint32_t layer,
   a.batch = batch;
   a.qscale = scale * kLog2e;
   a.window = window > 0 ? (uint32_t)window : 0;
-  return dtype == RVKV_F16 ? launch_decode<_Float16>(op, a, batch, pool->stream)
-                           : launch_decode<float>(op, a, batch, pool->stream);
+  return dtype == RVKV_F16
+             ? launch_decode<_Float16>(op, a, batch, w.waves, pool->stream)
+             : launch_decode<float>(op, a, batch, w.waves, pool->stream);
 }
 
 }  // extern "C"

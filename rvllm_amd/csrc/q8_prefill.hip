@@ -55,9 +55,6 @@ __device__ __forceinline__ float max_halves(float x) {
                                                   false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ uint32_t uniform(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
-}
 
 // Waves of a SIMD that the registers are bounded for.
 constexpr int waves_of(int hd, int cb) { return hd * cb > 128 ? 1 : 2; }

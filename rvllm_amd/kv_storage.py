@@ -46,8 +46,9 @@ def _dev_u32(x, device) -> torch.Tensor:
 
 
 def _on(store, op: str, tensors) -> None:
+    index = store.device.index if store.device.type == "cuda" else -1
     for t in tensors:
-        if t.device != store.device:
+        if t.get_device() != index:
             raise RvkvError(f"{op}: every tensor must be on the storage's "
                             "device")
 

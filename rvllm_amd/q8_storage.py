@@ -158,20 +158,31 @@ class HipQ8Storage:
 
     # -- attention ------------------------------------------------------------
     def _check_attn(self, op, q, out, ints):
-        _need(q.dim() == 3 and q.shape[2] == self.head_dim and
-              q.dtype in _DT and q.is_contiguous(),
-              f"{op}: q must be contiguous [rows, n_heads, head_dim] float32 "
-              "or float16")
+        shape, dtype = q.shape, q.dtype
+        if (len(shape) != 3 or shape[2] != self.head_dim or dtype not in _DT or
+                not q.is_contiguous()):
+            raise RvkvError(f"{op}: q must be contiguous [rows, n_heads, "
+                            "head_dim] float32 or float16")
         if out is None:
             out = torch.empty_like(q)
-        _need(out.shape == q.shape and out.dtype == q.dtype and
-              out.is_contiguous(), f"{op}: out must match q")
+        elif (out.shape != shape or out.dtype != dtype or
+              not out.is_contiguous()):
+            raise RvkvError(f"{op}: out must match q")
         for t in ints:
             if t.dtype != torch.int32 or not t.is_contiguous():
                 raise RvkvError(f"{op}: index tensors must be contiguous "
                                 "int32")
         _on(self, op, (q, out, *ints))
         return out
+
+    def _scratch(self, op, ws, need):
+        if ws is None:
+            return (torch.empty(need, dtype=torch.uint8, device=self.device)
+                    if need else None)
+        if ws.device != self.device or not ws.is_contiguous():
+            raise RvkvError(f"{op}: workspace must be contiguous and on the "
+                            "storage's device")
+        return ws
 
     def decode_workspace_bytes(self, batch: int, n_heads: int,
                                max_ctx_len: int, window: int = 0) -> int:
@@ -200,15 +211,19 @@ class HipQ8Storage:
               f"{op}: block_tables must be [batch, max_blocks]")
         _need(ctx_lens.numel() == batch,
               f"{op}: ctx_lens length must equal batch")
+        window = int(window or 0)
         if ws is None:
-            ws = self.alloc_workspace(batch, n_heads, max_ctx_len, window)
-        if scale is None:
-            scale = 1.0 / math.sqrt(hd)
+            ws = self._scratch(op, None, self.decode_workspace_bytes(
+                batch, n_heads, max_ctx_len, window))
+        else:
+            ws = self._scratch(op, ws, 0)
         check(self._L.rvkv_q8_paged_decode(
-            self._pool, layer, _ptr(q), _DT[q.dtype], _ptr(block_tables),
-            _ptr(ctx_lens), batch, block_tables.shape[1], n_heads, max_ctx_len,
-            float(scale), int(window or 0), _ptr(out), _ptr(ws),
-            ws.numel() * ws.element_size()))
+            self._pool, layer, q.data_ptr(), _DT[q.dtype],
+            block_tables.data_ptr(), ctx_lens.data_ptr(), batch,
+            block_tables.shape[1], n_heads, max_ctx_len,
+            1.0 / math.sqrt(hd) if scale is None else scale, window,
+            out.data_ptr(), None if ws is None else ws.data_ptr(),
+            0 if ws is None else ws.numel() * ws.element_size()))
         return out
 
     def prefill_workspace_bytes(self, rows: int, batch: int, n_heads: int,
@@ -241,16 +256,14 @@ class HipQ8Storage:
               f"{op}: pos_offset/read_num_tokens length must equal batch")
         rows, n_heads, hd = q.shape
         wide, window = int(block_tables.shape[1]), int(window or 0)
-        if scale is None:
-            scale = 1.0 / math.sqrt(hd)
-        if ws is None:
-            need = self.prefill_workspace_bytes(rows, batch, n_heads, wide,
-                                                window)
-            if need:
-                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws = self._scratch(op, ws, 0 if ws is not None else
+                           self.prefill_workspace_bytes(rows, batch, n_heads,
+                                                        wide, window))
         check(self._L.rvkv_q8_packed_prefill(
-            self._pool, layer, _ptr(q), _DT[q.dtype], _ptr(row_start), rows,
-            _ptr(block_tables), _ptr(pos_offset), _ptr(read_num_tokens),
-            batch, wide, n_heads, float(scale), window, _ptr(out), _ptr(ws),
+            self._pool, layer, q.data_ptr(), _DT[q.dtype],
+            row_start.data_ptr(), rows, block_tables.data_ptr(),
+            pos_offset.data_ptr(), read_num_tokens.data_ptr(), batch, wide,
+            n_heads, 1.0 / math.sqrt(hd) if scale is None else scale, window,
+            out.data_ptr(), None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel() * ws.element_size()))
         return out
