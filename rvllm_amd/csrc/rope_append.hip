@@ -96,26 +96,277 @@ __device__ __forceinline__ int quantise(double x, double s, double inv) {
   return (int)__builtin_fmin(__builtin_fmax(r, -127.0), 127.0);
 }
 
-template <bool VEC, int E, typename In>
-__device__ __forceinline__ void load_row(const In *p, In (&x)[E]) {
-  static_assert(VEC && E == 8, "eight elements by 16-byte loads");
-  constexpr int N = 16 / sizeof(In);
-#pragma unroll
-  for (int i = 0; i < E / N; ++i)
-    *reinterpret_cast<uint4 *>(x + i * N) =
-        *reinterpret_cast<const uint4 *>(p + i * N);
+// The largest, or the sum, of T lanes, in every one of them (T 4 to 32). Each
+// step adds the lanes' mirror image in twice as wide a group, by DPP.
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true);
+  const uint32_t hi =
+      __builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int T, typename F>
+__device__ __forceinline__ double over_lanes(double x, F f) {
+  x = f(x, dpp<0xb1>(x));             // quad_perm 1 0 3 2
+  x = f(x, dpp<0x4e>(x));             // quad_perm 2 3 0 1
+  if (T > 4) x = f(x, dpp<0x141>(x));  // row_half_mirror
+  if (T > 8) x = f(x, dpp<0x140>(x));  // row_mirror
+  if (T > 16) x = f(x, __shfl_xor(x, 16));
+  return x;
 }
 
-// One workgroup a token: its angles into LDS, then T lanes a head. VEC: a
-// lane owns 8 consecutive dims (T = hd / 8) and, in the half layout, loads
-// its partners' 8 too (they lie in the same lines). Otherwise 16 lanes a
-// head, lane l owning dims l, l + 16, ... (any hd, rot, stride, alignment).
-template <typename In, int CELL, int T, bool VEC>
+// 1 / sqrt(x) for x > 0, normal: the instruction's start, then two Newton
+// steps (each doubles its more than 20 bits).
+__device__ __forceinline__ double rsqrt64(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double e = __builtin_fma(-x * y, y, 1.0);
+    y = __builtin_fma(0.5 * y, e, y);
+  }
+  return y;
+}
+
+// Eight elements of a row, by 16-byte accesses.
+template <typename X>
+struct Vec8 {
+  typedef X type __attribute__((ext_vector_type(8), aligned(16)));
+};
+
+// The code of a value x that f32 holds as xf to within 2^-23 of itself, by the
+// product with inv = 1 / s to 2^-22: the quotient is off by less than 127 *
+// 2^-21 < 2^-14, so a rounding further than that from a border is the exact
+// one's, and the others (one in 4000 values) are made exactly. (A scale that
+// is no normal number gives a quotient that is not below the border.)
+__device__ __forceinline__ int code_of(float xf, double x, float s, float inv) {
+  const float t = xf * inv, r = __builtin_rintf(t);
+  if (__builtin_fabsf(t - r) < 0.5f - 0x1p-14f && s > 0x1p-100f)
+    return (int)__builtin_fminf(__builtin_fmaxf(r, -127.f), 127.f);
+  if (!(s > 0.f)) return 0;
+  return quantise(x, (double)s, 1.0 / (double)s);
+}
+
+// The wide form: R tokens a workgroup, T lanes a head (T >= hd / 8, lanes
+// behind the head idle), lane l owning dims 8 l .. 8 l + 7; in the half layout
+// it also loads its partners' 8 (they lie in the same lines). The workgroup's
+// threads share the tokens' angles out between them first. f16 q is turned in
+// f32 (its angles come from f64), k in f64: codes go by it.
+//
+// A token's V codes lie bs bytes apart, one byte a dim. With R 4, tokens in
+// consecutive slots, as prompts have them, put their four bytes of a dim into
+// one store.
+template <typename In, int CELL, int T, int R>
 __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
-  constexpr int E = VEC ? 8 : 16;
-  __shared__ double cs[128], sn[128];
-  const uint32_t row = blockIdx.x;
+  typedef typename Vec8<In>::type In8;
+  __shared__ double cs[R][128], sn[R][128];
+  const uint32_t row0 = blockIdx.x * R;
+  const uint32_t n_rows = a.rows - row0 < R ? a.rows - row0 : R;
   const uint32_t half = a.rot / 2;
+  for (uint32_t i = threadIdx.x; i < half * n_rows; i += 256) {
+    const uint32_t r = i / half, p = i - r * half;
+    double s, c;
+    sincos64((double)a.positions[row0 + r] * (double)a.inv_freq[p], s, c);
+    cs[r][p] = c * (double)a.factor;
+    sn[r][p] = s * (double)a.factor;
+  }
+  uint32_t blk[R], off[R];
+  bool ok[R], run = R > 1 && n_rows == R;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool have = (uint32_t)r < n_rows;
+    blk[r] = have ? a.slot_block[row0 + r] : 0xffffffffu;
+    off[r] = have ? a.slot_off[row0 + r] : 0;
+    ok[r] = blk[r] < a.num_blocks && off[r] < a.bs;
+    run = run && ok[r] && blk[r] == blk[0] && off[r] == off[0] + r;
+  }
+  __syncthreads();
+  const uint32_t lane = threadIdx.x % T, hd = a.hd, d0 = 8 * lane;
+  const uint32_t n_slots = a.n_heads + 2 * a.n_kv;
+  const bool mine = d0 < hd;
+  const uint32_t dl = mine ? d0 : 0;  // (idle lanes load what lane 0 does)
+  for (uint32_t slot = threadIdx.x / T; slot < n_slots; slot += 256 / T) {
+    const bool is_q = slot < a.n_heads;
+    const bool is_v = slot >= a.n_heads + a.n_kv;
+    const uint32_t hh = is_q ? slot
+                             : (is_v ? slot - a.n_heads - a.n_kv
+                                     : slot - a.n_heads);
+    const uint64_t stride = is_q ? a.q_stride : (is_v ? a.v_stride : a.k_stride);
+    const In *src = (const In *)(is_q ? a.q : (is_v ? a.v : a.k)) +
+                    row0 * stride + (size_t)hh * hd;
+    const float *w = is_v ? nullptr : (is_q ? a.q_norm : a.k_norm);
+    const bool turn = !is_v && dl < a.rot;
+    const bool is_a = dl < half;
+    const uint32_t d1 = !turn || a.interleaved ? dl
+                                               : (is_a ? dl + half : dl - half);
+    const uint32_t p0 = a.interleaved ? dl / 2 : (is_a ? dl : d1);
+    float wx[8], wy[8];
+    if (w) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        wx[e] = w[dl + e];
+        wy[e] = w[d1 + e];
+      }
+    }
+    In8 own[R], other[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t rr = (uint32_t)r < n_rows ? r : 0;
+      own[r] = *reinterpret_cast<const In8 *>(src + rr * stride + dl);
+      other[r] = own[r];
+      if (turn && !a.interleaved)
+        other[r] = *reinterpret_cast<const In8 *>(src + rr * stride + d1);
+    }
+    uint32_t vcode[8] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if ((uint32_t)r >= n_rows) break;
+      double norm = 1.0;
+      if (w) {
+        double ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double x = (double)own[r][e];
+          ss = __builtin_fma(x, x, ss);
+        }
+        ss = over_lanes<T>(mine ? ss : 0.0,
+                           [](double x, double y) { return x + y; });
+        norm = rsqrt64(ss / (double)hd + (double)a.eps);
+      }
+      if (is_q && sizeof(In) == 2) {
+        float x[8];
+        const float nf = (float)norm;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[e] = w ? (float)own[r][e] * nf * wx[e] : (float)own[r][e];
+        if (turn && a.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float c = (float)cs[r][p0 + e / 2];
+            const float s = (float)sn[r][p0 + e / 2];
+            const float u = x[e], v = x[e + 1];
+            x[e] = u * c - v * s;
+            x[e + 1] = u * s + v * c;
+          }
+        } else if (turn) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = w ? (float)other[r][e] * nf * wy[e]
+                              : (float)other[r][e];
+            const float s = (float)sn[r][p0 + e];
+            x[e] = __builtin_fmaf(x[e], (float)cs[r][p0 + e],
+                                  is_a ? -y * s : y * s);
+          }
+        }
+        In8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (In)x[e];
+        if (mine)
+          *reinterpret_cast<In8 *>(
+              (In *)a.q_out + ((size_t)(row0 + r) * a.n_heads + hh) * hd + d0) =
+              y;
+        continue;
+      }
+      double x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = w ? (double)own[r][e] * norm * (double)wx[e]
+                 : (double)own[r][e];
+      if (turn && a.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const double c = cs[r][p0 + e / 2], s = sn[r][p0 + e / 2];
+          const double u = x[e], v = x[e + 1];
+          x[e] = u * c - v * s;
+          x[e + 1] = u * s + v * c;
+        }
+      } else if (turn) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double y = w ? (double)other[r][e] * norm * (double)wy[e]
+                             : (double)other[r][e];
+          const double s = is_a ? -sn[r][p0 + e] : sn[r][p0 + e];
+          x[e] = x[e] * cs[r][p0 + e] + y * s;
+        }
+      }
+      const auto put = [&](auto *out) {
+        using Out = typename std::remove_pointer<decltype(out)>::type;
+        typename Vec8<Out>::type y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          Out z;
+          round_to(x[e], z);
+          y[e] = z;
+        }
+        if (mine)
+          *reinterpret_cast<typename Vec8<Out>::type *>(out + d0) = y;
+      };
+      if (is_q) {
+        put((In *)a.q_out + ((size_t)(row0 + r) * a.n_heads + hh) * hd);
+        continue;
+      }
+      unsigned char *block = (is_v ? a.vc : a.kc) + (ok[r] ? blk[r] : 0) * a.rec;
+      const size_t row_at = (size_t)hh * a.bs + off[r];
+      if (CELL != kQ8) {
+        if (ok[r]) {
+          if (CELL == kF16) put((_Float16 *)block + row_at * hd);
+          else put((float *)block + row_at * hd);
+        }
+        continue;
+      }
+      double top = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double m = __builtin_fabs(x[e]);
+        // (a NaN counts as infinite: the row is then not finite)
+        top = m <= top ? top : (m == m ? m : __builtin_inf());
+      }
+      top = over_lanes<T>(mine ? top : 0.0, [](double u, double v) {
+        return __builtin_fmax(u, v);
+      });
+      const float scale = top < __builtin_inf() ? (float)(top / 127.0)
+                                                : __builtin_nanf("");
+      const float inv = __builtin_amdgcn_rcpf(scale);
+      uint32_t code[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        code[e] = (uint32_t)code_of((float)x[e], x[e], scale, inv) & 255;
+      if (!ok[r]) continue;
+      if (lane == 0)
+        *reinterpret_cast<float *>(block + (size_t)a.n_kv * a.bs * hd +
+                                   row_at * 4) = scale;
+      if (!is_v) {
+        if (mine)
+          *reinterpret_cast<uint2 *>(block + row_at * hd + d0) = uint2{
+              code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+              code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+        continue;
+      }
+      if (run) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vcode[e] |= code[e] << (8 * (r & 3));
+      } else if (mine) {
+        unsigned char *v = block + ((size_t)hh * hd + d0) * a.bs + off[r];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[(size_t)e * a.bs] = (unsigned char)code[e];
+      }
+    }
+    if (CELL == kQ8 && run && is_v && mine) {
+      unsigned char *v =
+          a.vc + blk[0] * a.rec + ((size_t)hh * hd + d0) * a.bs + off[0];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // (any alignment)
+        __builtin_memcpy(v + (size_t)e * a.bs, &vcode[e], 4);
+    }
+  }
+}
+
+// The plain form, for any rot, stride and alignment: one token a workgroup,
+// 16 lanes a head, lane l owning dims l, l + 16, ...
+template <typename In, int CELL>
+__global__ void __launch_bounds__(256) rope_append_any_kernel(RopeArgs a) {
+  __shared__ double cs[128], sn[128];
+  const uint32_t row = blockIdx.x, hd = a.hd, half = a.rot / 2;
   for (uint32_t p = threadIdx.x; p < half; p += 256) {
     double s, c;
     sincos64((double)a.positions[row] * (double)a.inv_freq[p], s, c);
@@ -124,176 +375,105 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
   }
   __syncthreads();
   const uint32_t blk = a.slot_block[row], off = a.slot_off[row];
-  const bool slot_ok = blk < a.num_blocks && off < a.bs;
-  const uint32_t lane = threadIdx.x % T;
+  const bool ok = blk < a.num_blocks && off < a.bs;
+  const uint32_t lane = threadIdx.x % 16;
   const uint32_t n_slots = a.n_heads + 2 * a.n_kv;
-  const uint32_t hd = a.hd;
-  for (uint32_t slot = threadIdx.x / T; slot < n_slots; slot += 256 / T) {
+  for (uint32_t slot = threadIdx.x / 16; slot < n_slots; slot += 16) {
     const bool is_q = slot < a.n_heads;
     const bool is_v = slot >= a.n_heads + a.n_kv;
     const uint32_t hh = is_q ? slot
                              : (is_v ? slot - a.n_heads - a.n_kv
                                      : slot - a.n_heads);
-    if (!is_q && !slot_ok) continue;
-    const In *src = is_q ? (const In *)a.q + (size_t)row * a.q_stride
-                         : (is_v ? (const In *)a.v + (size_t)row * a.v_stride
-                                 : (const In *)a.k + (size_t)row * a.k_stride);
+    if (!is_q && !ok) continue;
+    const In *src = is_q ? (const In *)a.q + row * a.q_stride
+                         : (is_v ? (const In *)a.v + row * a.v_stride
+                                 : (const In *)a.k + row * a.k_stride);
     src += (size_t)hh * hd;
     const float *w = is_v ? nullptr : (is_q ? a.q_norm : a.k_norm);
-    const auto dim = [&](int e) {
-      return VEC ? 8 * lane + e : lane + 16 * (uint32_t)e;
-    };
-    double x[E];
-    if constexpr (VEC) {
-      alignas(16) In own[E];
-      load_row<VEC, E>(src + 8 * lane, own);
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = (double)own[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = dim(e) < hd ? (double)src[dim(e)] : 0.0;
-    }
     double norm = 1.0;
-    if (w) {  // (uniform over a head's lanes)
+    if (w) {
       double ss = 0.0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) ss = __builtin_fma(x[e], x[e], ss);
-#pragma unroll
-      for (int o = T / 2; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, T);
-      norm = 1.0 / sqrt(ss / (double)hd + (double)a.eps);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (VEC || dim(e) < hd) x[e] = x[e] * norm * (double)w[dim(e)];
-    }
-    if (!is_v && a.rot) {
-      if constexpr (VEC) {
-        const uint32_t d0 = 8 * lane;
-        if (d0 < a.rot) {
-          if (a.interleaved) {
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-              const double c = cs[(d0 + e) / 2], s = sn[(d0 + e) / 2];
-              const double u = x[e], v = x[e + 1];
-              x[e] = u * c - v * s;
-              x[e + 1] = u * s + v * c;
-            }
-          } else {
-            const bool is_a = d0 < half;
-            const uint32_t d1 = is_a ? d0 + half : d0 - half;
-            const uint32_t p0 = is_a ? d0 : d1;
-            alignas(16) In other[E];
-            load_row<VEC, E>(src + d1, other);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              double y = (double)other[e];
-              if (w) y = y * norm * (double)w[d1 + e];
-              const double s = is_a ? -sn[p0 + e] : sn[p0 + e];
-              x[e] = x[e] * cs[p0 + e] + y * s;
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t d = dim(e);
-          if (d < a.rot) {
-            const bool is_a = a.interleaved ? !(d & 1) : d < half;
-            const uint32_t p = a.interleaved ? d >> 1 : (is_a ? d : d - half);
-            const uint32_t d1 = a.interleaved ? d ^ 1
-                                              : (is_a ? d + half : d - half);
-            double y = (double)src[d1];
-            if (w) y = y * norm * (double)w[d1];
-            x[e] = x[e] * cs[p] + y * (is_a ? -sn[p] : sn[p]);
-          }
-        }
+      for (uint32_t d = lane; d < hd; d += 16) {
+        const double x = (double)src[d];
+        ss = __builtin_fma(x, x, ss);
       }
+      ss = over_lanes<16>(ss, [](double x, double y) { return x + y; });
+      norm = rsqrt64(ss / (double)hd + (double)a.eps);
     }
-    if (is_q || CELL != kQ8) {
-      // q in its own type, or a row of f16 / f32 cells.
-      const auto put = [&](auto *out) {
-        using Out = typename std::remove_pointer<decltype(out)>::type;
-        if constexpr (VEC) {
-          alignas(16) Out y[E];
+    double x[16], top = 0.0;
 #pragma unroll
-          for (int e = 0; e < E; ++e) round_to(x[e], y[e]);
-          constexpr int N = 16 / sizeof(Out);
-#pragma unroll
-          for (int i = 0; i < E / N; ++i)
-            *reinterpret_cast<uint4 *>(out + 8 * lane + i * N) =
-                *reinterpret_cast<const uint4 *>(y + i * N);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (dim(e) < hd) round_to(x[e], out[dim(e)]);
-        }
-      };
-      if (is_q) {
-        put((In *)a.q_out + ((size_t)row * a.n_heads + hh) * hd);
-      } else {
-        unsigned char *block = (is_v ? a.vc : a.kc) + blk * a.rec;
-        const size_t at = ((size_t)hh * a.bs + off) * hd;
-        if (CELL == kF16) put((_Float16 *)block + at);
-        else put((float *)block + at);
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t d = lane + 16 * e;
+      x[e] = 0.0;
+      if (d >= hd) continue;
+      x[e] = w ? (double)src[d] * norm * (double)w[d] : (double)src[d];
+      if (!is_v && d < a.rot) {
+        const bool is_a = a.interleaved ? !(d & 1) : d < half;
+        const uint32_t p = a.interleaved ? d >> 1 : (is_a ? d : d - half);
+        const uint32_t d1 = a.interleaved ? d ^ 1 : (is_a ? d + half : d - half);
+        const double y = w ? (double)src[d1] * norm * (double)w[d1]
+                           : (double)src[d1];
+        x[e] = x[e] * cs[p] + y * (is_a ? -sn[p] : sn[p]);
       }
-      continue;
-    }
-    double top = 0.0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
       const double m = __builtin_fabs(x[e]);
-      // (a NaN counts as infinite: the row is then not finite)
       top = m <= top ? top : (m == m ? m : __builtin_inf());
     }
+    unsigned char *block = (is_v ? a.vc : a.kc) + (ok ? blk : 0) * a.rec;
+    const size_t row_at = (size_t)hh * a.bs + off;
+    const auto put = [&](auto *out) {
 #pragma unroll
-    for (int o = T / 2; o >= 1; o >>= 1)
-      top = __builtin_fmax(top, __shfl_xor(top, o, T));
-    const float scale = top < __builtin_inf() ? (float)(top / 127.0)
-                                              : __builtin_nanf("");
-    const double s = (double)scale, inv = 1.0 / s;
-    int code[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      code[e] = scale > 0.f ? quantise(x[e], s, inv) : 0;
-    unsigned char *block = (is_v ? a.vc : a.kc) + blk * a.rec;
-    unsigned char *tile = block + (size_t)hh * a.bs * hd;
-    if (is_v) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (VEC || dim(e) < hd)
-          tile[(size_t)dim(e) * a.bs + off] = (unsigned char)code[e];
-    } else if constexpr (VEC) {
-      uint2 pack;
-      pack.x = (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 |
-               (uint32_t)code[3] << 24;
-      pack.y = (code[4] & 255) | (code[5] & 255) << 8 | (code[6] & 255) << 16 |
-               (uint32_t)code[7] << 24;
-      *reinterpret_cast<uint2 *>(tile + (size_t)off * hd + 8 * lane) = pack;
+      for (int e = 0; e < 16; ++e)
+        if (lane + 16 * e < hd) round_to(x[e], out[lane + 16 * e]);
+    };
+    if (is_q) {
+      put((In *)a.q_out + ((size_t)row * a.n_heads + hh) * hd);
+    } else if (CELL == kF16) {
+      put((_Float16 *)block + row_at * hd);
+    } else if (CELL == kF32) {
+      put((float *)block + row_at * hd);
     } else {
+      top = over_lanes<16>(top, [](double u, double v) {
+        return __builtin_fmax(u, v);
+      });
+      const float scale = top < __builtin_inf() ? (float)(top / 127.0)
+                                                : __builtin_nanf("");
+      const double s = (double)scale, inv = 1.0 / s;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (dim(e) < hd)
-          tile[(size_t)off * hd + dim(e)] = (unsigned char)code[e];
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t d = lane + 16 * e;
+        if (d < hd)
+          block[is_v ? ((size_t)hh * hd + d) * a.bs + off : row_at * hd + d] =
+              (unsigned char)(scale > 0.f ? quantise(x[e], s, inv) : 0);
+      }
+      if (lane == 0)
+        *reinterpret_cast<float *>(block + (size_t)a.n_kv * a.bs * hd +
+                                   row_at * 4) = scale;
     }
-    if (lane == 0)
-      *reinterpret_cast<float *>(block + (size_t)a.n_kv * a.bs * hd +
-                                 ((size_t)hh * a.bs + off) * 4) = scale;
   }
 }
 
+// Four tokens a workgroup from 2048 on, where they fill the chip.
+template <typename In, int CELL, int T>
+void launch_wide(const RopeArgs &a, hipStream_t st) {
+  if (a.rows >= 2048)
+    hipLaunchKernelGGL((rope_append_kernel<In, CELL, T, 4>),
+                       dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((rope_append_kernel<In, CELL, T, 1>), dim3(a.rows),
+                       dim3(256), 0, st, a);
+}
+
 template <typename In, int CELL>
-void launch(const RopeArgs &a, bool vec, hipStream_t st) {
-  const dim3 grid(a.rows), block(256);
-  if (vec) {
-    switch (a.hd) {
-      case 32: hipLaunchKernelGGL((rope_append_kernel<In, CELL, 4, true>), grid, block, 0, st, a); return;
-      case 64: hipLaunchKernelGGL((rope_append_kernel<In, CELL, 8, true>), grid, block, 0, st, a); return;
-      case 128: hipLaunchKernelGGL((rope_append_kernel<In, CELL, 16, true>), grid, block, 0, st, a); return;
-      case 256: hipLaunchKernelGGL((rope_append_kernel<In, CELL, 32, true>), grid, block, 0, st, a); return;
-      default: break;
-    }
-  }
-  hipLaunchKernelGGL((rope_append_kernel<In, CELL, 16, false>), grid, block, 0,
-                     st, a);
+void launch(const RopeArgs &a, bool wide, hipStream_t st) {
+  if (!wide)
+    hipLaunchKernelGGL((rope_append_any_kernel<In, CELL>), dim3(a.rows),
+                       dim3(256), 0, st, a);
+  else if (a.hd <= 64)
+    launch_wide<In, CELL, 8>(a, st);
+  else if (a.hd <= 128)
+    launch_wide<In, CELL, 16>(a, st);
+  else
+    launch_wide<In, CELL, 32>(a, st);
 }
 
 // The checks that both pools' entry points share; fills a.
@@ -326,8 +506,8 @@ int rope_append(const char *op, int cell, hipStream_t st, RopeArgs &a,
       (uintptr_t)a.q_out % eb)
     return fail(RVKV_EINVAL, op, "q/k/v/q_out must be aligned to their type");
   a.interleaved = interleaved;
-  bool vec = a.hd == 32 || a.hd == 64 || a.hd == 128 || a.hd == 256;
-  vec = vec && (interleaved ? a.rot % 8 == 0 : a.rot % 16 == 0);
+  bool vec = a.hd % 8 == 0 &&
+             (interleaved ? a.rot % 8 == 0 : a.rot % 16 == 0);
   for (uint64_t x : {(uint64_t)(uintptr_t)a.q, (uint64_t)(uintptr_t)a.k,
                      (uint64_t)(uintptr_t)a.v, (uint64_t)(uintptr_t)a.q_out,
                      a.q_stride * eb, a.k_stride * eb, a.v_stride * eb})

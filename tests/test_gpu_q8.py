@@ -51,6 +51,8 @@ APPENDS = [
     (2, 1, 16, 16, 16, False, "f32", 3, True),
     (8, 2, 64, 16, 24, False, "f16", 19, True),     # rot / 2 not in eights
     (8, 2, 64, 16, 0, False, "f16", 19, True),      # no rotation
+    (4, 2, 128, 16, 128, False, "f16", 2050, True),  # four tokens a workgroup
+    (3, 1, 80, 32, 48, True, "f32", 2051, True),
 ]
 
 
@@ -81,11 +83,13 @@ def test_q8_rope_append(H, kv, hd, bs, rot, inter, dtype, rows, fused, norm):
     eps = float(np.float32(1e-6))
     want_q = ref.rotate(q, pos, inv, inter, f32f, wq, eps)
     want_k = ref.rotate(k, pos, inv, inter, f32f, wk, eps)
-    # q is rounded once: half a step of its type (and 2^-40 of the largest
-    # value of its row for the f64 sums and angles, far below it)
+    # q is rounded once: half a step of its type, and for the sums and angles
+    # before it 2^-40 of its row's largest value in f64, 2^-21 (eight roundings
+    # of 2^-24: angles, norm, weight, products, sum) where f16 q takes f32
+    before = 2.0 ** (-21 if q.dtype == torch.float16 else -40)
     room = (torch.finfo(q.dtype).eps / 2 * 1.0001 * want_q.abs()
             + 2.0 ** -24 * torch.finfo(q.dtype).tiny
-            + 2.0 ** -40 * want_q.abs().amax(-1, keepdim=True)
+            + before * want_q.abs().amax(-1, keepdim=True)
             + (2.0 ** -25 if q.dtype == torch.float16 else 0))
     assert ((got.cpu().double() - want_q).abs() <= room).all()
     for which, x in ((0, want_k), (1, v.double().cpu())):
@@ -117,6 +121,7 @@ def test_rope_append_into_f16_and_f32_pools(H, kv, hd, bs, rot, inter, dtype,
     want_q = ref.rotate(q, pos, inv, inter, 1.0)
     assert ((got.cpu().double() - want_q).abs()
             <= torch.finfo(q.dtype).eps / 2 * 1.0001 * want_q.abs()
+            + 2.0 ** -21 * want_q.abs().amax(-1, keepdim=True)
             + 2.0 ** -24).all()
     for which, x in ((0, ref.rotate(k, pos, inv, inter, 1.0)),
                      (1, v.double().cpu())):
@@ -167,6 +172,29 @@ def test_q8_append_skips_slots_out_of_range():
     assert left[2, :, 5].all()
     left[2, :, 5] = 0
     assert not left.any()
+
+
+@pytest.mark.parametrize("first", [0, 1, 3, 14])
+def test_q8_append_runs_of_slots(first):
+    """Prompts in consecutive slots from any offset on, block ends inside a
+    group of four tokens, a slot out of range and one out of order."""
+    kv, hd, bs, rows = 2, 64, 16, 2052
+    nb = rows // bs + 2
+    st = HipQ8Storage(1, nb, bs, kv, hd)
+    k, v = randn((rows, kv, hd), 1), randn((rows, kv, hd), 2)
+    at = first + np.arange(rows)
+    at[[100, 101]] = at[[101, 100]]
+    blk, off = at // bs, at % bs
+    blk[333] = nb
+    st.write_tokens(0, i32(blk), i32(off), k, v)
+    keep = np.arange(rows) != 333
+    for which, x in ((0, k), (1, v)):
+        codes, scale = ref.quantise(x.double().cpu()[keep])
+        assert torch.equal(st.codes(0, which).cpu()[blk[keep], :, off[keep]],
+                           codes)
+        assert torch.equal(st.scales(0, which).cpu()[blk[keep], :, off[keep]],
+                           scale)
+        assert (st.scales(0, which) != 0).sum() == (rows - 1) * kv
 
 
 # -- decode -------------------------------------------------------------------
