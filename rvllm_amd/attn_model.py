@@ -32,7 +32,8 @@ import torch
 from . import _lib
 from ._lib import check
 from .kv_storage import HipDecodePlan, HipKvStorage
-from .rope import rope_cos_sin
+from .q8_storage import HipQ8Storage
+from .rope import rope_cos_sin, rope_inv_freq
 
 
 @dataclass
@@ -90,10 +91,17 @@ def padded_tables(items) -> np.ndarray:
 
 
 class HipBackend:
-    """Engine backend (forward_sample / release / copy_blocks) on one GPU."""
+    """Engine backend (forward_sample / release / copy_blocks) on one GPU.
+    cache: "f16", or "q8" for the 8-bit cache (half the bytes): attention prep
+    is then rvkv_q8_rope_append, a forward's prompts are one
+    rvkv_q8_packed_prefill a layer and a decode batch one
+    rvkv_q8_paged_decode."""
 
     def __init__(self, cfg: AttnModelConfig, weights: Dict[str, np.ndarray],
-                 num_blocks: int, block_size: int, device: str = "cuda"):
+                 num_blocks: int, block_size: int, device: str = "cuda",
+                 cache: str = "f16"):
+        if cache not in ("f16", "q8"):
+            raise ValueError(f"cache must be f16 or q8, not {cache}")
         self.cfg = cfg
         self.config = SimpleNamespace(context_length=cfg.context_length)
         self.dev = torch.device(device)
@@ -108,8 +116,9 @@ class HipBackend:
             if cfg.qkv_bias:
                 self.w[f"bqkv{l}"] = torch.cat(
                     [self.w[f"bq{l}"], self.w[f"bk{l}"], self.w[f"bv{l}"]])
-        self.st = HipKvStorage(cfg.n_layers, num_blocks, block_size,
-                               cfg.n_kv_heads, cfg.head_dim)
+        self.q8 = cache == "q8"
+        self.st = (HipQ8Storage if self.q8 else HipKvStorage)(
+            cfg.n_layers, num_blocks, block_size, cfg.n_kv_heads, cfg.head_dim)
         self._L = _lib.load()
         self.last_logits = None
         self.forwards = 0
@@ -122,8 +131,12 @@ class HipBackend:
         # RoPE rows of every position the model takes, on the GPU; a forward
         # gathers its own (computing 1700 rows' angles on the host took 0.9 ms
         # a forward). 2^17 positions take 0.2-0.3 s here, once.
-        self._rope = self._rope_rows(np.arange(min(cfg.context_length,
-                                                   1 << 17)))
+        if self.q8:  # (angles come from positions)
+            self._inv_freq = torch.from_numpy(rope_inv_freq(
+                cfg.rope_theta, cfg.head_dim)).to(self.dev)
+        else:
+            self._rope = self._rope_rows(np.arange(min(cfg.context_length,
+                                                       1 << 17)))
 
     def _rope_rows(self, pos) -> tuple:
         """cos and sin of the positions' angles, on the GPU."""
@@ -174,6 +187,9 @@ class HipBackend:
             chain.from_iterable(chain.from_iterable(
                 it.write_positions for it in items)),
             np.uint32).reshape(-1, 2)
+        if self.q8:
+            return self._forward_q8(items, last_only, n_new, toks, pos, slots,
+                                    first, last)
         rope = None
         if rows and int(pos.max()) >= self._rope[0].shape[0]:
             rope = self._rope_rows(pos)  # (past the table: these rows alone)
@@ -219,12 +235,51 @@ class HipBackend:
                                      scale=scale, window=c.window)
                     r0 += n
             x = x + att.view(rows, H * hd) @ w[f"wo{l}"]
-        xs = x[last]
+        return self._pick(x[last], len(items))
+
+    def _forward_q8(self, items, last_only, n_new, toks, pos, slots, first,
+                    last) -> List[int]:
+        c, w, st = self.cfg, self.w, self.st
+        H, KV, hd, rows = c.n_heads, c.n_kv_heads, c.head_dim, len(toks)
+        reads = np.array([it.read_num_tokens for it in items], np.int64)
+        longest = int(reads.max())
+        starts = np.concatenate([[0], np.cumsum(n_new)])
+        toks, pos, sb, so, tables, offs, reads, last, starts = self._send(
+            [toks, pos, slots[:, 0], slots[:, 1], padded_tables(items), first,
+             reads, last, starts])
+        decode = not last_only and bool((n_new == 1).all())
+        # One workspace a forward, shared by its layers (they run in turn).
+        need = (st.decode_workspace_bytes(rows, H, longest, c.window)
+                if decode else st.prefill_workspace_bytes(
+                    rows, len(items), H, tables.shape[1], c.window))
+        ws = torch.empty(need, dtype=torch.uint8,
+                         device=self.dev) if need else None
+        x = w["embed"][toks]
+        for l in range(c.n_layers):
+            qkv = x @ w[f"wqkv{l}"]
+            if c.qkv_bias:
+                qkv += w[f"bqkv{l}"]
+            q, k, v = (t.view(rows, -1, hd) for t in
+                       qkv.split([H * hd, KV * hd, KV * hd], dim=1))
+            q = st.rope_append(l, q, k, v, pos, self._inv_freq, sb, so,
+                               q_norm=w.get(f"qn{l}"), k_norm=w.get(f"kn{l}"),
+                               eps=c.eps)
+            if decode:
+                att = st.paged_decode(l, q, tables, reads, longest, ws=ws,
+                                      window=c.window)
+            else:
+                att = st.packed_prefill(l, q, starts, tables, offs, reads,
+                                        ws=ws, window=c.window)
+            x = x + att.view(rows, H * hd) @ w[f"wo{l}"]
+        return self._pick(x[last], len(items))
+
+    def _pick(self, xs, n: int) -> List[int]:
+        c, w, st = self.cfg, self.w, self.st
         logits = (xs @ w["embed"].T) * logit_scale(c)
         logits = logits.contiguous()
-        ids = torch.empty(len(items), dtype=torch.int32, device=self.dev)
+        ids = torch.empty(n, dtype=torch.int32, device=self.dev)
         check(self._L.rvkv_argmax(ctypes.c_void_p(logits.data_ptr()),
-                                  len(items), c.vocab,
+                                  n, c.vocab,
                                   ctypes.c_void_p(ids.data_ptr()),
                                   ctypes.c_void_p(st.stream.cuda_stream)))
         self.last_logits = logits

@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2)
       }
       if (more) load_k(pk1);
       if (masked) {
-        asm volatile("");  // (a branch, no selects on every tile)
+        __builtin_amdgcn_sched_barrier(0);  // (a branch, no selects on every tile)
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = keep >> j & 1 ? s[j] : kNone;
       }
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2)
       vtop = max_wave(vtop);
       if (__any(top > m) || vtop >= __uint_as_float((uint32_t)(142 - shift)
                                                     << 23)) {
-        asm volatile("");
+        __builtin_amdgcn_sched_barrier(0);
         const float now = fmaxf(m, top);
         float fix = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
         m = now;

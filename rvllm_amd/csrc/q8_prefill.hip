@@ -19,7 +19,6 @@
 //
 // f16 rows take q as it is and round the weights p vs once to f16. f32 rows
 // take q and the weights as two f16 parts each, twice the products.
-#include <cstdlib>
 #include "q8.h"
 
 using rvkv_detail::fail;
@@ -28,7 +27,7 @@ using rvkv_detail::kMaxKeys;
 
 namespace {
 
-constexpr int kKeys = 64;
+constexpr int kRows = 128, kKeys = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PackedArgs {
@@ -55,9 +54,6 @@ __device__ __forceinline__ float max_halves(float x) {
                                                   false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-
-// Waves of a SIMD that the registers are bounded for.
-constexpr int waves_of(int hd, int cb) { return hd * cb > 128 ? 1 : 2; }
 
 template <int HD>
 struct alignas(16) Tile {
@@ -104,7 +100,6 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 // More sequences: one behind the other, b owning indices row_start[b] * group
 // / 128 + b onward, at least as many as it has tiles; the host's n_tiles
 // counts in that way.
-template <int kRows>
 __device__ __forceinline__ bool find_work(const PackedArgs &a, uint32_t t,
                                           Work &w) {
   const uint32_t lane = threadIdx.x & 63, G = a.group;
@@ -205,10 +200,10 @@ __device__ __forceinline__ bool find_work(const PackedArgs &a, uint32_t t,
   return true;
 }
 
-template <typename T, int HD, bool SPLIT, int CB>
-__global__ void __launch_bounds__(256, waves_of(HD, CB))
+template <typename T, int HD, bool SPLIT>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     q8_prefill_kernel(PackedArgs a) {
-  constexpr int NC = HD / 16, ND = HD / 32, kRows = 128 * CB;
+  constexpr int NC = HD / 16, ND = HD / 32;
   constexpr int KPT = HD / 64;  // 16-byte chunks of K, and of V, a thread
   constexpr float kNone = -__builtin_inff();
   extern __shared__ __align__(16) unsigned char smem[];
@@ -222,7 +217,7 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
   const uint32_t piece = rest % a.n_pieces;
   const uint32_t t = rest / a.n_pieces;
   Work w;
-  if (!find_work<kRows>(a, t, w)) return;
+  if (!find_work(a, t, w)) return;
   uint32_t beg = w.beg, end = w.end;
   bool whole = true;  // this workgroup sees all its rows' keys
   if (a.n_pieces > 1) {
@@ -237,32 +232,27 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
     }
   }
 
-  // This lane's q rows, and the keys [key_lo, key_lo + span) that each sees.
-  bool live[CB];
-  size_t row[CB];
-  uint32_t key_lo[CB], span[CB];
+  // This lane's q row, and the keys [key_lo, key_lo + span) that it sees.
   uint32_t all_lo = 0, all_hi = 0xffffffffu, any_lo = 0xffffffffu, any_hi = 0;
-#pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const uint32_t f = w.f0 + (wave * CB + b) * 32 + col;
-    live[b] = f < w.n_flat;
-    const uint32_t fl = live[b] ? f : w.f0, tok = fl / G;
-    const uint32_t head = kvh * G + (fl - tok * G);
-    row[b] = ((size_t)(w.r0 + tok) * a.n_heads + head) * hd;
-    const uint64_t pos = w.pos0 + tok;
-    const uint32_t key_hi = (uint32_t)(pos + 1 < w.read ? pos + 1 : w.read);
-    key_lo[b] = a.window && pos + 1 > a.window
-                    ? (uint32_t)(pos + 1 - a.window < w.read
-                                     ? pos + 1 - a.window : w.read) : 0;
-    span[b] = live[b] && key_hi > key_lo[b] ? key_hi - key_lo[b] : 0;
-    if (live[b]) {
-      all_lo = max(all_lo, key_lo[b]);
-      all_hi = min(all_hi, key_hi);
-    }
-    if (span[b]) {
-      any_lo = min(any_lo, key_lo[b]);
-      any_hi = max(any_hi, key_hi);
-    }
+  const uint32_t f = w.f0 + wave * 32 + col;
+  const bool live = f < w.n_flat;
+  const uint32_t fl = live ? f : w.f0, tok = fl / G;
+  const uint32_t head = kvh * G + (fl - tok * G);
+  const size_t row = ((size_t)(w.r0 + tok) * a.n_heads + head) * hd;
+  const uint64_t pos = w.pos0 + tok;
+  const uint32_t key_hi = (uint32_t)(pos + 1 < w.read ? pos + 1 : w.read);
+  const uint32_t key_lo =
+      a.window && pos + 1 > a.window
+          ? (uint32_t)(pos + 1 - a.window < w.read ? pos + 1 - a.window
+                                                   : w.read) : 0;
+  const uint32_t span = live && key_hi > key_lo ? key_hi - key_lo : 0;
+  if (live) {
+    all_lo = max(all_lo, key_lo);
+    all_hi = min(all_hi, key_hi);
+  }
+  if (span) {
+    any_lo = min(any_lo, key_lo);
+    any_hi = max(any_hi, key_hi);
   }
   // Keys that every row of this wave sees, and that any does.
 #pragma unroll
@@ -381,79 +371,66 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
 
   // q: element j of chunk c is dim 16 c + 8 h + j. rf: what a score is still
   // to be multiplied by.
-  half8v qh[CB][NC], ql[SPLIT ? CB : 1][SPLIT ? NC : 1];
-  float rf[CB];
+  half8v qh[NC], ql[SPLIT ? NC : 1];
+  float rf = 1.f;
+  const T *q = (const T *)a.q + row;
+  if constexpr (!SPLIT) {
 #pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const T *q = (const T *)a.q + row[b];
-    rf[b] = 1.f;
-    if constexpr (!SPLIT) {
+    for (int c = 0; c < NC; ++c)
+      qh[c] = live && (uint32_t)c * 16 < hd
+                     ? *reinterpret_cast<const half8v *>(q + c * 16 + 8 * h)
+                     : half8v{};
+  } else {
+    // (brought just below 2^15 by a power of two: neither part leaves f16's
+    // range, the lower one not its normal numbers)
+    float x[NC][8];
+    float top = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        qh[b][c] = live[b] && (uint32_t)c * 16 < hd
-                       ? *reinterpret_cast<const half8v *>(q + c * 16 + 8 * h)
-                       : half8v{};
-    } else {
-      // (brought just below 2^15 by a power of two: neither part leaves f16's
-      // range, the lower one not its normal numbers)
-      float x[NC][8];
-      float top = 0.f;
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int j = 0; j < 8; ++j) {
+        x[c][j] = live && (uint32_t)c * 16 < hd
+                      ? (float)q[c * 16 + 8 * h + j] : 0.f;
+        top = fmaxf(top, fabsf(x[c][j]));
+      }
+    top = max_halves(top);
+    const uint32_t ex = scale_exponent(top);
+    const float down = __uint_as_float((269 - ex) << 23);
+    rf = __uint_as_float((ex - 15) << 23);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[c][j] = live[b] && (uint32_t)c * 16 < hd
-                        ? (float)q[c * 16 + 8 * h + j] : 0.f;
-          top = fmaxf(top, fabsf(x[c][j]));
-        }
-      top = max_halves(top);
-      const uint32_t ex = scale_exponent(top);
-      const float down = __uint_as_float((269 - ex) << 23);
-      rf[b] = __uint_as_float((ex - 15) << 23);
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y = x[c][j] * down;
-          qh[b][c][j] = (_Float16)y;
-          ql[b][c][j] = (_Float16)(y - (float)qh[b][c][j]);
-        }
-    }
+      for (int j = 0; j < 8; ++j) {
+        const float y = x[c][j] * down;
+        qh[c][j] = (_Float16)y;
+        ql[c][j] = (_Float16)(y - (float)qh[c][j]);
+      }
   }
 
   // m: what the weights are relative to, their maximum to within 2^8 (it
   // moves, and o and l with it, only when a score passes it by more).
-  float m[CB], l[CB];
+  float m = kNone, l = 0.f;
   float vnorm = kVnorm0;
-  float16v o[CB][ND];
+  float16v o[ND];
 #pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    m[b] = kNone;
-    l[b] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[b][d] = float16v{};
-  }
+  for (int d = 0; d < ND; ++d) o[d] = float16v{};
   const uint32_t key_row = 16 * (col >> 4) + 8 * ((col >> 2) & 1) +
                            4 * ((col >> 3) & 1) + (col & 3);
 
   const auto step = [&](const Tile<HD> &s, uint32_t kt) {
-    float16v sc[CB][2];
+    float16v sc[2];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
-#pragma unroll
-      for (int b = 0; b < CB; ++b) sc[b][kh] = float16v{};
+      sc[kh] = float16v{};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const half8v kf = *reinterpret_cast<const half8v *>(
             &s.k[kh * 32 + key_row][c * 16 + 8 * h]);
-#pragma unroll
-        for (int b = 0; b < CB; ++b) {
-          sc[b][kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              kf, qh[b][c], sc[b][kh], 0, 0, 0);
-          if constexpr (SPLIT)
-            sc[b][kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                kf, ql[b][c], sc[b][kh], 0, 0, 0);
-        }
+        sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+            kf, qh[c], sc[kh], 0, 0, 0);
+        if constexpr (SPLIT)
+          sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              kf, ql[c], sc[kh], 0, 0, 0);
       }
     }
     // Register 8 u + j of half kh: key 32 kh + 16 u + 8 h + j.
@@ -466,62 +443,50 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
         const float4v k4 = *reinterpret_cast<const float4v *>(
             &s.ks[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int b = 0; b < CB; ++b) sc[b][kh][r + i] *= k4[i];
+        for (int i = 0; i < 4; ++i) sc[kh][r + i] *= k4[i];
       }
     if (masked) {  // (uniform over the wave)
-      asm volatile("");  // (a branch, no selects on every tile)
-#pragma unroll
-      for (int b = 0; b < CB; ++b) {
-        const uint32_t from = kt + 8 * h - key_lo[b];
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const uint32_t key = from + kh * 32 + 16 * (r >> 3) + (r & 7);
-            sc[b][kh][r] = key < span[b] ? sc[b][kh][r] : kNone;
-            if (bad >> (2 * kh + (r >> 3)) & 1) sc[b][kh][r] = kNone;
-          }
-      }
-    }
-    float fix[CB], mm[CB];
-    bool any_fix = false;
-#pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      float top = kNone;
+      __builtin_amdgcn_sched_barrier(0);  // (a branch, no selects on every tile)
+      const uint32_t from = kt + 8 * h - key_lo;
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2)
-          top = fmaxf(fmaxf(sc[b][kh][r], sc[b][kh][r + 1]), top);
-      top = max_halves(top);
-      if constexpr (SPLIT) top *= rf[b];
-      fix[b] = 1.f;
-      if (__any(top > m[b] + 8.f)) {
-        const float now = fmaxf(m[b], top);
-        // (-inf less -inf: nothing was seen, and nothing is held)
-        fix[b] = m[b] == now ? 1.f : __builtin_amdgcn_exp2f(m[b] - now);
-        m[b] = now;
-        l[b] *= fix[b];
-        any_fix = true;
-      }
-      mm[b] = m[b] == kNone ? 0.f : m[b];
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t key = from + kh * 32 + 16 * (r >> 3) + (r & 7);
+          sc[kh][r] = key < span ? sc[kh][r] : kNone;
+          if (bad >> (2 * kh + (r >> 3)) & 1) sc[kh][r] = kNone;
+        }
     }
-    if (s.vnorm != vnorm) {  // (uniform)
+    float fix = 1.f;
+    bool any_fix = false;
+    float top = kNone;
 #pragma unroll
-      for (int b = 0; b < CB; ++b) fix[b] *= vnorm / s.vnorm;
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        top = fmaxf(fmaxf(sc[kh][r], sc[kh][r + 1]), top);
+    top = max_halves(top);
+    if constexpr (SPLIT) top *= rf;
+    if (__any(top > m + 8.f)) {
+      const float now = fmaxf(m, top);
+      // (-inf less -inf: nothing was seen, and nothing is held)
+      fix = m == now ? 1.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= fix;
+      any_fix = true;
+    }
+    const float mm = m == kNone ? 0.f : m;
+    if (s.vnorm != vnorm) {  // (uniform)
+      fix *= vnorm / s.vnorm;
       vnorm = s.vnorm;
       any_fix = true;
     }
     if (any_fix) {
-      asm volatile("");
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < CB; ++b)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[b][d] *= fix[b];
+      for (int d = 0; d < ND; ++d) o[d] *= fix;
     }
-    half8v ph[CB][4], pl[SPLIT ? CB : 1][SPLIT ? 4 : 1];
+    half8v ph[4], pl[SPLIT ? 4 : 1];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
@@ -530,32 +495,30 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
             &s.vs[kh * 32 + 16 * (r >> 3) + 8 * h + (r & 7)]);
         const int x = 2 * kh + (r >> 3);
 #pragma unroll
-        for (int b = 0; b < CB; ++b)
+        for (int i = 0; i < 4; i += 2) {
+          float y[2];
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            float y[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float p = __builtin_amdgcn_exp2f(
-                  SPLIT ? __builtin_fmaf(sc[b][kh][r + i + e], rf[b], -mm[b])
-                        : sc[b][kh][r + i + e] - mm[b]);
-              l[b] += p;
-              // (0 for a key that is left out, whatever its scale holds)
-              y[e] = rvkv_mul0(p, v4[i + e]);
-            }
-            const int at = (r & 7) + i;
-            if constexpr (SPLIT) {
-              const half2v u = pk(y[0], y[1]);
-              const half2v v = pk(y[0] - (float)u[0], y[1] - (float)u[1]);
-              ph[b][x][at] = u[0];
-              ph[b][x][at + 1] = u[1];
-              pl[b][x][at] = v[0];
-              pl[b][x][at + 1] = v[1];
-            } else {
-              ph[b][x][at] = (_Float16)y[0];
-              ph[b][x][at + 1] = (_Float16)y[1];
-            }
+          for (int e = 0; e < 2; ++e) {
+            const float p = __builtin_amdgcn_exp2f(
+                SPLIT ? __builtin_fmaf(sc[kh][r + i + e], rf, -mm)
+                      : sc[kh][r + i + e] - mm);
+            l += p;
+            // (0 for a key that is left out, whatever its scale holds)
+            y[e] = rvkv_mul0(p, v4[i + e]);
           }
+          const int at = (r & 7) + i;
+          if constexpr (SPLIT) {
+            const half2v u = pk(y[0], y[1]);
+            const half2v v = pk(y[0] - (float)u[0], y[1] - (float)u[1]);
+            ph[x][at] = u[0];
+            ph[x][at + 1] = u[1];
+            pl[x][at] = v[0];
+            pl[x][at + 1] = v[1];
+          } else {
+            ph[x][at] = (_Float16)y[0];
+            ph[x][at + 1] = (_Float16)y[1];
+          }
+        }
       }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -563,14 +526,11 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
       for (int x = 0; x < 4; ++x) {
         const half8v vf = *reinterpret_cast<const half8v *>(
             &s.v[d * 32 + col][x * 16 + 8 * h]);
-#pragma unroll
-        for (int b = 0; b < CB; ++b) {
-          o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              vf, ph[b][x], o[b][d], 0, 0, 0);
-          if constexpr (SPLIT)
-            o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                vf, pl[b][x], o[b][d], 0, 0, 0);
-        }
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+            vf, ph[x], o[d], 0, 0, 0);
+        if constexpr (SPLIT)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              vf, pl[x], o[d], 0, 0, 0);
       }
   };
 
@@ -592,57 +552,54 @@ __global__ void __launch_bounds__(256, waves_of(HD, CB))
   }
 
   const float back = vnorm * 0x1p-6f;
+  l += __shfl_xor(l, 32);
+  if (!whole) {
+    // A piece's part: o and l relative to m, for the merge.
+    const size_t slot =
+        ((size_t)(t * a.n_kv + kvh) * a.n_pieces + piece) * kRows +
+        wave * 32 + col;
+    float *to = a.ws_acc + slot * HD;
 #pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    l[b] += __shfl_xor(l[b], 32);
-    if (!whole) {
-      // A piece's part: o and l relative to m, for the merge.
-      const size_t slot =
-          ((size_t)(t * a.n_kv + kvh) * a.n_pieces + piece) * kRows +
-          (wave * CB + b) * 32 + col;
-      float *to = a.ws_acc + slot * HD;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
+      for (int r = 0; r < 16; r += 4) {
+        float4v y;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          float4v y;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = o[b][d][r + i] * back;
-          *reinterpret_cast<float4v *>(to + d * 32 + 2 * r + 4 * h) = y;
-        }
-      if (h == 0) {
-        a.ws_ml[2 * slot] = m[b];
-        a.ws_ml[2 * slot + 1] = l[b];
+        for (int i = 0; i < 4; ++i) y[i] = o[d][r + i] * back;
+        *reinterpret_cast<float4v *>(to + d * 32 + 2 * r + 4 * h) = y;
       }
-    } else if (live[b]) {
-      T *out = (T *)a.out + row[b];
-      const float inv = l[b] == 0.f ? 0.f : back / l[b];
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const uint32_t dim = d * 32 + 2 * r + 4 * h;
-          if (dim < hd) {
-            typedef T vec4 __attribute__((ext_vector_type(4)));
-            vec4 y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = (T)(o[b][d][r + i] * inv);
-            *reinterpret_cast<vec4 *>(out + dim) = y;
-          }
-        }
+    if (h == 0) {
+      a.ws_ml[2 * slot] = m;
+      a.ws_ml[2 * slot + 1] = l;
     }
+  } else if (live) {
+    T *out = (T *)a.out + row;
+    const float inv = l == 0.f ? 0.f : back / l;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const uint32_t dim = d * 32 + 2 * r + 4 * h;
+        if (dim < hd) {
+          typedef T vec4 __attribute__((ext_vector_type(4)));
+          vec4 y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = (T)(o[d][r + i] * inv);
+          *reinterpret_cast<vec4 *>(out + dim) = y;
+        }
+      }
   }
 }
 
 // Merges the pieces of tiles that were cut: 32 rows a workgroup, HD / 4
 // threads a row.
-template <typename T, int HD, int kRows>
+template <typename T, int HD>
 __global__ void __launch_bounds__(256) q8_prefill_reduce_kernel(PackedArgs a) {
   constexpr float kNone = -__builtin_inff();
   constexpr uint32_t TR = HD / 4;
   const uint32_t kvh = blockIdx.x % a.n_kv, t = blockIdx.x / a.n_kv;
   Work w;
-  if (!find_work<kRows>(a, t, w)) return;
+  if (!find_work(a, t, w)) return;
   if (w.end <= w.beg || w.end - w.beg <= a.piece_keys) return;
   const uint32_t live = (w.end - w.beg - 1) / a.piece_keys + 1;
   const uint32_t d = threadIdx.x % TR * 4;
@@ -680,38 +637,25 @@ __global__ void __launch_bounds__(256) q8_prefill_reduce_kernel(PackedArgs a) {
 uint32_t hd_up(uint32_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 struct Layout {
-  uint32_t rows;  // of a tile
   uint64_t n_tiles, n_pieces, piece_keys;
   size_t ml_off, bytes;
 };
-
-// Tiles of 256 rows, 64 a wave: a K or V operand read from LDS feeds two
-// products and a tile's conversion serves twice the rows, at one wave a SIMD.
-bool wide_rows(const rvkv_q8_pool *p, uint64_t n_tiles, rvkv_dtype dtype) {
-  return dtype == RVKV_F16 && p->head_dim <= 128 &&
-         n_tiles * p->n_kv >= 1024 && getenv("WIDE");
-}
 
 // How a call is cut. The rows' tiles alone where they give every CU its
 // workgroups (two up to hd 128, one above); otherwise each tile's keys, as far
 // as the host can tell them from the width of the table and the window, in
 // pieces of at least 128.
 Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
-              uint32_t n_heads, uint32_t max_blocks, uint32_t window,
-              rvkv_dtype dtype) {
+              uint32_t n_heads, uint32_t max_blocks, uint32_t window) {
   Layout w{};
   const uint32_t G = n_heads / p->n_kv;
   const uint64_t want = p->head_dim > 128 ? 256 : 512;
-  w.rows = 128;
-  w.n_tiles = (uint64_t)total_rows * G / w.rows + batch;
+  w.n_tiles = (uint64_t)total_rows * G / kRows + batch;
   w.n_pieces = 1;
-  if (wide_rows(p, w.n_tiles, dtype)) {
-    w.rows = 256;
-    w.n_tiles = (uint64_t)total_rows * G / w.rows + batch;
-  }
+
   uint64_t keys = (uint64_t)max_blocks * p->block_size;
   if (keys > kMaxKeys) keys = kMaxKeys;
-  const uint64_t band = (uint64_t)window + w.rows / G + 16;
+  const uint64_t band = (uint64_t)window + kRows / G + 16;
   if (window && band < keys) keys = band;
   w.piece_keys = keys;
   const uint64_t have = w.n_tiles * p->n_kv;
@@ -722,43 +666,34 @@ Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
   if (n < 2) return w;
   w.piece_keys = ((keys + n - 1) / n + kKeys - 1) / kKeys * kKeys;
   w.n_pieces = (keys + w.piece_keys - 1) / w.piece_keys;
-  const size_t rows = (size_t)have * w.n_pieces * w.rows;
+  const size_t rows = (size_t)have * w.n_pieces * kRows;
   w.ml_off = rows * hd_up(p->head_dim) * 4;
   w.bytes = (w.ml_off + rows * 8 + 255) & ~(size_t)255;
   return w;
 }
 
-template <typename T, int HD, bool SPLIT, int CB>
+template <typename T, int HD, bool SPLIT>
 int launch(const char *op, const PackedArgs &a, hipStream_t st) {
   const size_t lds = 2 * sizeof(Tile<HD>);
   static const hipError_t set = hipFuncSetAttribute(
-      reinterpret_cast<const void *>(&q8_prefill_kernel<T, HD, SPLIT, CB>),
+      reinterpret_cast<const void *>(&q8_prefill_kernel<T, HD, SPLIT>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (set != hipSuccess) return hip_fail(op, set);
-  hipLaunchKernelGGL((q8_prefill_kernel<T, HD, SPLIT, CB>),
+  hipLaunchKernelGGL((q8_prefill_kernel<T, HD, SPLIT>),
                      dim3(a.n_tiles * a.n_kv * a.n_pieces), dim3(256), lds, st,
                      a);
   if (a.n_pieces > 1)
-    hipLaunchKernelGGL((q8_prefill_reduce_kernel<T, HD, 128 * CB>),
-                       dim3(a.n_tiles * a.n_kv, 4 * CB), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((q8_prefill_reduce_kernel<T, HD>),
+                       dim3(a.n_tiles * a.n_kv, 4), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
 }
 
-int launch_f16(const char *op, const PackedArgs &a, uint32_t rows,
-               hipStream_t st) {
-  if (a.hd > 128) return launch<_Float16, 256, false, 1>(op, a, st);
-  if (a.hd > 64)
-    return rows == 256 ? launch<_Float16, 128, false, 2>(op, a, st)
-                       : launch<_Float16, 128, false, 1>(op, a, st);
-  return rows == 256 ? launch<_Float16, 64, false, 2>(op, a, st)
-                     : launch<_Float16, 64, false, 1>(op, a, st);
-}
-
-int launch_f32(const char *op, const PackedArgs &a, hipStream_t st) {
-  if (a.hd > 128) return launch<float, 256, true, 1>(op, a, st);
-  if (a.hd > 64) return launch<float, 128, true, 1>(op, a, st);
-  return launch<float, 64, true, 1>(op, a, st);
+template <typename T, bool SPLIT>
+int launch(const char *op, const PackedArgs &a, hipStream_t st) {
+  if (a.hd <= 64) return launch<T, 64, SPLIT>(op, a, st);
+  if (a.hd <= 128) return launch<T, 128, SPLIT>(op, a, st);
+  return launch<T, 256, SPLIT>(op, a, st);
 }
 
 }  // namespace
@@ -770,9 +705,8 @@ size_t rvkv_q8_prefill_workspace_bytes(const rvkv_q8_pool *pool,
                                        uint32_t n_heads, uint32_t max_blocks,
                                        int32_t window) {
   if (!pool || n_heads == 0 || n_heads % pool->n_kv) return 0;
-  // (calls that are cut have too few rows for the tiles to go by the type)
   return layout(pool, total_rows, batch, n_heads, max_blocks,
-                window > 0 ? (uint32_t)window : 0, RVKV_F32).bytes;
+                window > 0 ? (uint32_t)window : 0).bytes;
 }
 
 int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
@@ -804,7 +738,7 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
     return fail(RVKV_EINVAL, op, "q and out must be 16-byte aligned");
   const uint32_t bsg = pool->block_size / 16;
   const uint32_t win = window > 0 ? (uint32_t)window : 0;
-  Layout w = layout(pool, total_rows, batch, n_heads, max_blocks, win, dtype);
+  Layout w = layout(pool, total_rows, batch, n_heads, max_blocks, win);
   if (!ws) w.n_pieces = 1;
   if (w.n_pieces > 1 && ws_bytes < w.bytes)
     return fail(RVKV_EINVAL, op, "workspace smaller than the required bytes");
@@ -842,8 +776,8 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
   a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.ml_off);
   a.bsg_log2 = bsg & (bsg - 1) ? -1 : __builtin_ctz(bsg);
   a.qscale = scale * kLog2e;
-  return dtype == RVKV_F16 ? launch_f16(op, a, w.rows, pool->stream)
-                           : launch_f32(op, a, pool->stream);
+  return dtype == RVKV_F16 ? launch<_Float16, false>(op, a, pool->stream)
+                           : launch<float, true>(op, a, pool->stream);
 }
 
 }  // extern "C"

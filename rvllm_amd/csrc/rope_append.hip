@@ -477,8 +477,8 @@ void launch(const RopeArgs &a, bool wide, hipStream_t st) {
 }
 
 // The checks that both pools' entry points share; fills a.
-int rope_append(const char *op, int cell, hipStream_t st, RopeArgs &a,
-                rvkv_dtype dtype, uint32_t interleaved) {
+int rope_append(const char *op, int cell, int device, hipStream_t st,
+                RopeArgs &a, rvkv_dtype dtype, uint32_t interleaved) {
   if (dtype != RVKV_F16 && dtype != RVKV_F32)
     return fail(RVKV_EINVAL, op, "dtype must be F16 or F32");
   if (!a.k || !a.v || !a.slot_block || !a.slot_off)
@@ -505,6 +505,8 @@ int rope_append(const char *op, int cell, hipStream_t st, RopeArgs &a,
   if ((uintptr_t)a.q % eb || (uintptr_t)a.k % eb || (uintptr_t)a.v % eb ||
       (uintptr_t)a.q_out % eb)
     return fail(RVKV_EINVAL, op, "q/k/v/q_out must be aligned to their type");
+  const int rc = rvkv_detail::q8_device(op, device);
+  if (rc) return rc;
   a.interleaved = interleaved;
   bool vec = a.hd % 8 == 0 &&
              (interleaved ? a.rot % 8 == 0 : a.rot % 16 == 0);
@@ -572,8 +574,6 @@ int rvkv_rope_append(rvkv_pool *pool, uint32_t layer, const void *q,
   if (layer >= pool->n_layers)
     return fail(RVKV_EINVAL, op, "layer out of range");
   if (rows == 0) return RVKV_OK;
-  const int rc = rvkv_detail::q8_device(op, pool->device);
-  if (rc) return rc;
   RopeArgs a = rope_args(q, q_stride, k, k_stride, v, v_stride, rows, n_heads,
                          q_norm, k_norm, eps, positions, inv_freq, rot_dim,
                          attn_factor, slot_block, slot_off, q_out);
@@ -584,8 +584,8 @@ int rvkv_rope_append(rvkv_pool *pool, uint32_t layer, const void *q,
   a.kc = reinterpret_cast<unsigned char *>(pool->tensor(layer, 0));
   a.vc = reinterpret_cast<unsigned char *>(pool->tensor(layer, 1));
   a.rec = pool->block16 * 2;
-  return rope_append(op, pool->f32() ? kF32 : kF16, pool->stream, a, dtype,
-                     interleaved);
+  return rope_append(op, pool->f32() ? kF32 : kF16, pool->device,
+                     pool->stream, a, dtype, interleaved);
 }
 
 int rvkv_q8_rope_append(rvkv_q8_pool *pool, uint32_t layer, const void *q,
@@ -602,8 +602,6 @@ int rvkv_q8_rope_append(rvkv_q8_pool *pool, uint32_t layer, const void *q,
   if (layer >= pool->n_layers)
     return fail(RVKV_EINVAL, op, "layer out of range");
   if (rows == 0) return RVKV_OK;
-  const int rc = rvkv_detail::q8_device(op, pool->device);
-  if (rc) return rc;
   RopeArgs a = rope_args(q, q_stride, k, k_stride, v, v_stride, rows, n_heads,
                          q_norm, k_norm, eps, positions, inv_freq, rot_dim,
                          attn_factor, slot_block, slot_off, q_out);
@@ -614,7 +612,8 @@ int rvkv_q8_rope_append(rvkv_q8_pool *pool, uint32_t layer, const void *q,
   a.kc = pool->tensor(layer, 0);
   a.vc = pool->tensor(layer, 1);
   a.rec = pool->rec;
-  return rope_append(op, kQ8, pool->stream, a, dtype, interleaved);
+  return rope_append(op, kQ8, pool->device, pool->stream, a, dtype,
+                     interleaved);
 }
 
 }  // extern "C"

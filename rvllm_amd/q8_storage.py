@@ -95,12 +95,16 @@ class HipQ8Storage:
             rec, bs, hd = self._record(), self.block_size, self.head_dim
             nb, kv = self.num_blocks, self.n_kv_heads
             first = (2 * layer + which) * nb * rec
-            codes = self.memory.view(torch.int8).as_strided(
+            # (as_strided counts from the storage's start, not the tensor's)
+            bytes_, words = (self.memory[:self.nbytes].view(t) for t in
+                             (torch.int8, torch.float32))
+            codes = bytes_.as_strided(
                 (nb, kv, bs, hd),
-                (rec, bs * hd) + ((hd, 1) if which == 0 else (1, bs)), first)
-            scales = self.memory[:self.nbytes].view(torch.float32).as_strided(
+                (rec, bs * hd) + ((hd, 1) if which == 0 else (1, bs)),
+                bytes_.storage_offset() + first)
+            scales = words.as_strided(
                 (nb, kv, bs), (rec // 4, bs, 1),
-                (first + kv * bs * hd) // 4)
+                words.storage_offset() + (first + kv * bs * hd) // 4)
             got = self._views[layer, which] = codes, scales
         return got
 

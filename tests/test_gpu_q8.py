@@ -518,3 +518,159 @@ def test_q8_append_then_prompt_then_decode():
         for b in (0, 1):
             w, tol = want(b, q[b:b + 1], pos[b])
             ref.check_close(out[b:b + 1], w, tol, "decode")
+
+
+# -- streams, graphs ----------------------------------------------------------
+
+def test_q8_graph_replays_like_eager():
+    """Append, packed prompts and decode captured into one graph on a stream
+    of its own; replayed beside eager work, each replay with new inputs gives
+    the eager bits."""
+    H, kv, hd, bs, n = 8, 2, 64, 16, 150
+    nb = 40
+    st, eager = (HipQ8Storage(1, nb, bs, kv, hd) for _ in range(2))
+    inv = inv_freq(hd)
+    table = i32([list(range(0, 12)), list(range(12, 24))])
+    pos = np.concatenate([np.arange(n), np.arange(n)])
+    blk = i32(np.concatenate([pos[:n] // bs, pos[n:] // bs + 12]))
+    off, pos = i32(pos % bs), i32(pos)
+    starts, zero, reads = i32([0, n, 2 * n]), i32([0, 0]), i32([n, n])
+    x = randn((2 * n, (H + 2 * kv) * hd), 1).half()
+    out = torch.empty((2 * n, H, hd), dtype=torch.float16, device="cuda")
+    dec = torch.empty((2, H, hd), dtype=torch.float16, device="cuda")
+    qo = torch.empty_like(out)
+    wsp = torch.empty(max(256, st.prefill_workspace_bytes(2 * n, 2, H, 12)),
+                      dtype=torch.uint8, device="cuda")
+    wsd = st.alloc_workspace(2, H, n)
+
+    def run(s, o, d):
+        q, k, v = (t.view(2 * n, -1, hd) for t in
+                   x.split([H * hd, kv * hd, kv * hd], dim=1))
+        s.rope_append(0, q, k, v, pos, inv, blk, off, q_out=qo)
+        s.packed_prefill(0, qo, starts, table, zero, reads, out=o, ws=wsp)
+        s.paged_decode(0, o[:2], table, reads, n, out=d, ws=wsd)
+
+    run(st, out, dec)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        st.set_stream(torch.cuda.current_stream())
+        run(st, out, dec)
+    st.set_stream(torch.cuda.current_stream())
+    for seed in range(4):
+        x.copy_(randn(x.shape, 50 + seed).half())
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        o2, d2 = torch.empty_like(out), torch.empty_like(dec)
+        run(eager, o2, d2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, o2) and torch.equal(dec, d2)
+        assert torch.equal(st.codes(0, 1), eager.codes(0, 1))
+
+
+def test_q8_pool_on_its_own_stream():
+    """Calls run on the pool's stream, whatever torch's current one is."""
+    side = torch.cuda.Stream()
+    st = filled(40, 16, 2, 64, 3)
+    q, table, ctx = randn((2, 4, 64), 1), i32([[3, 5, 7], [9, 11, 2]]), i32(
+        [40, 33])
+    want = st.paged_decode(0, q, table, ctx, 48)
+    torch.cuda.synchronize()
+    st.set_stream(side)
+    got = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    st.paged_decode(0, q, table, ctx, 48, out=got)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_q8_two_calls_at_once_with_their_own_workspaces():
+    """Two pools' decodes on two streams, many partitions each."""
+    a, b = filled(300, 16, 2, 64, 3), filled(300, 16, 2, 64, 4)
+    table, ctx = i32([list(range(300))]), i32([4800])
+    q = randn((1, 8, 64), 1)
+    want = [s.paged_decode(0, q, table, ctx, 4800) for s in (a, b)]
+    ws = [s.alloc_workspace(1, 8, 4800) for s in (a, b)]
+    outs = [[torch.empty_like(q) for _ in range(8)] for _ in (a, b)]
+    torch.cuda.synchronize()
+    for s in (a, b):
+        s.set_stream(torch.cuda.Stream())
+    for i in range(8):
+        for s, w, o in zip((a, b), ws, outs):
+            s.paged_decode(0, q, table, ctx, 4800, out=o[i], ws=w)
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(x, w) for x in o)
+
+
+# -- the engine's backend -----------------------------------------------------
+
+def engine_items(rng, vocab, lens, bs, width):
+    from rvllm_amd.engine import BatchItem
+    items = []
+    for i, n in enumerate(lens):
+        blocks = list(range(i * width, i * width + width))
+        items.append(BatchItem(i, rng.integers(0, vocab, n).tolist(),
+                               [(blocks[p // bs], p % bs) for p in range(n)],
+                               blocks, n, 0))
+    return items
+
+
+@pytest.mark.parametrize("variant", ["plain", "norm", "bias", "window"])
+def test_q8_backend_forward(variant):
+    """Prompts in one forward give each prompt's own logits, and a decode step
+    those of the prompt with its token (a row's cells depend on the row
+    alone): the same f32 computation in another order of sums. Two layers of
+    f32 products of 128: 1e-4 of the logits' size is far above their
+    rounding."""
+    from rvllm_amd.attn_model import AttnModelConfig, HipBackend, init_weights
+    from rvllm_amd.engine import BatchItem
+    cfg = AttnModelConfig(vocab=256, hidden=128, n_layers=2, n_heads=8,
+                          n_kv_heads=2, head_dim=64,
+                          qkv_bias=variant == "bias",
+                          qk_norm=variant == "norm",
+                          window=24 if variant == "window" else 0)
+    w = init_weights(cfg)
+    rng = np.random.default_rng(1)
+    items = engine_items(rng, cfg.vocab, [40, 7, 99], 16, 8)
+    be = HipBackend(cfg, w, 30, 16, cache="q8")
+    ids = be.forward_sample(items, True, [None] * 3)
+    packed = be.last_logits.clone()
+    size = packed.abs().max().item()
+    for i, it in enumerate(items):
+        alone = HipBackend(cfg, w, 30, 16, cache="q8")
+        assert alone.forward_sample([it], True, [None]) == [ids[i]]
+        assert (alone.last_logits[0] - packed[i]).abs().max() < 1e-4 * size
+    step = [BatchItem(it.seq_id, [t], [(it.read_blocks[n // 16], n % 16)],
+                      it.read_blocks, n + 1, n)
+            for it, t in zip(items, ids) for n in [len(it.tokens)]]
+    be.forward_sample(step, False, [None] * 3)
+    for i, (it, t) in enumerate(zip(items, ids)):
+        n = len(it.tokens) + 1
+        whole = HipBackend(cfg, w, 30, 16, cache="q8")
+        whole.forward_sample(
+            [BatchItem(0, it.tokens + [t],
+                       [(it.read_blocks[p // 16], p % 16) for p in range(n)],
+                       it.read_blocks, n, 0)], True, [None])
+        assert (whole.last_logits[0] - be.last_logits[i]).abs().max() \
+            < 1e-4 * size
+
+
+def test_q8_engine_runs_with_preemption_and_prefix_hits():
+    """The engine over the 8-bit backend: preempted requests and shared
+    prefixes end with the tokens of an engine with room for all."""
+    from rvllm_amd.attn_model import AttnModelConfig, HipBackend, init_weights
+    from rvllm_amd.engine import EngineConfig, RequestSpec, run
+    cfg = AttnModelConfig(vocab=512, hidden=128, n_layers=2, n_heads=8,
+                          n_kv_heads=2, head_dim=64, context_length=512)
+    w = init_weights(cfg)
+    rng = np.random.default_rng(5)
+    shared = rng.integers(0, 512, 40).tolist()
+    reqs = [RequestSpec((shared if i % 2 == 0 else []) + rng.integers(
+        0, 512, 10 + i).tolist(), 12 + i) for i in range(6)]
+    got = [run(HipBackend(cfg, w, n, 16, cache="q8"), reqs,
+               EngineConfig(16, n, max_running=6)) for n in (12, 100)]
+    assert got[0].generated == got[1].generated
+    assert got[0].stats.preemptions > 0 and got[0].stats.prefix_hits > 0
