@@ -532,7 +532,7 @@ uint32_t rvkv_sched_refcount(const rvkv_sched *s, uint32_t block);
  * (F16 or F32), rows q_stride, k_stride, v_stride elements apart, heads of a
  * row one behind the other (so slices of a fused QKV buffer are taken in
  * place). The rotated q goes to q_out [rows, n_heads, head_dim] of dtype,
- * which must not overlap the inputs; n_heads 0: no q (q and q_out may be
+ * which must not overlap q, k or v (RVKV_EINVAL); n_heads 0: no q (q and q_out may be
  * NULL). k and v go to (slot_block[i], slot_off[i]) of `layer`; slots must be
  * distinct within a call; a row whose slot is out of range still gives its
  * q_out. positions, inv_freq (f32 [rot_dim / 2]), slots: device. head_dim <=
@@ -570,8 +570,8 @@ typedef struct rvkv_q8_pool rvkv_q8_pool;
 size_t rvkv_q8_pool_bytes(uint32_t n_layers, uint32_t num_blocks,
                           uint32_t block_size, uint32_t n_kv_heads,
                           uint32_t head_dim);
-/* memory: device memory of at least rvkv_q8_pool_bytes(...) bytes, 256-byte
- * aligned, that outlives the pool and is used as it is (a cache can be kept
+/* memory: memory of the current device, at least rvkv_q8_pool_bytes(...)
+ * bytes, 256-byte aligned, that outlives the pool and is used as it is (a cache can be kept
  * or shared that way); NULL: the pool allocates its own, zeroed. */
 int rvkv_q8_pool_create(uint32_t n_layers, uint32_t num_blocks,
                         uint32_t block_size, uint32_t n_kv_heads,

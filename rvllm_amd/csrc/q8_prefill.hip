@@ -19,6 +19,13 @@
 //
 // f16 rows take q as it is and round the weights p vs once to f16. f32 rows
 // take q and the weights as two f16 parts each, twice the products.
+//
+// Bound by issue: a tile of 64 keys costs a wave its matrix cycles (1024 at hd
+// 128) and then its vector cycles (softmax, conversion, staging: ~1600), which
+// overlap little. Seven prompts of 571 to 4001 rows, 16 + 8 heads of 128: 187
+// GFLOP in 284 us, 660 TFLOP/s; 4 prompts up to 4000 at 32 + 8 heads of 64: 555.
+// With 64 rows a wave, each LDS operand feeding two products, the accumulators
+// move between the register files every tile: 514 us.
 #include "q8.h"
 
 using rvkv_detail::fail;
@@ -591,8 +598,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   }
 }
 
-// Merges the pieces of tiles that were cut: 32 rows a workgroup, HD / 4
-// threads a row.
+// Merges the pieces of tiles that were cut: HD / 4 threads a row, one row each.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) q8_prefill_reduce_kernel(PackedArgs a) {
   constexpr float kNone = -__builtin_inff();
@@ -603,8 +609,8 @@ __global__ void __launch_bounds__(256) q8_prefill_reduce_kernel(PackedArgs a) {
   if (w.end <= w.beg || w.end - w.beg <= a.piece_keys) return;
   const uint32_t live = (w.end - w.beg - 1) / a.piece_keys + 1;
   const uint32_t d = threadIdx.x % TR * 4;
-  for (uint32_t r = threadIdx.x / TR; r < 32; r += 256 / TR) {
-    const uint32_t in = blockIdx.y * 32 + r;
+  {
+    const uint32_t in = blockIdx.y * (256 / TR) + threadIdx.x / TR;
     const uint32_t f = w.f0 + in;
     if (f >= w.n_flat) return;
     const size_t slot0 = (size_t)(t * a.n_kv + kvh) * a.n_pieces * kRows + in;
@@ -641,15 +647,20 @@ struct Layout {
   size_t ml_off, bytes;
 };
 
-// How a call is cut. The rows' tiles alone where they give every CU its
-// workgroups (two up to hd 128, one above); otherwise each tile's keys, as far
-// as the host can tell them from the width of the table and the window, in
-// pieces of at least 128.
+// How a call is cut: into the workgroups that are resident at once (256 CUs by
+// two, by three at hd 64 in f16, by one above hd 128). The rows' tiles alone
+// where they are at least half of that; otherwise each tile's keys as well, as
+// far as the host can tell them from the width of the table and the window, in
+// pieces of at least 128. 450 rows behind 7700 keys, 32 + 8 heads of 64: f32
+// 109 us for 512 workgroups, 164 for 256, 137 for 768; f16 74 us for 768, 83
+// for 512, 136 for 256.
 Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
-              uint32_t n_heads, uint32_t max_blocks, uint32_t window) {
+              uint32_t n_heads, uint32_t max_blocks, uint32_t window,
+              rvkv_dtype dtype) {
   Layout w{};
   const uint32_t G = n_heads / p->n_kv;
-  const uint64_t want = p->head_dim > 128 ? 256 : 512;
+  const uint64_t want = p->head_dim > 128 ? 256
+                        : p->head_dim <= 64 && dtype == RVKV_F16 ? 768 : 512;
   w.n_tiles = (uint64_t)total_rows * G / kRows + batch;
   w.n_pieces = 1;
 
@@ -660,7 +671,7 @@ Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
   w.piece_keys = keys;
   const uint64_t have = w.n_tiles * p->n_kv;
   if (have == 0 || have * 2 > want) return w;
-  uint64_t n = want / have;
+  uint64_t n = (want + have - 1) / have;
   if (n > (keys + 127) / 128) n = (keys + 127) / 128;
   if (n > 16) n = 16;
   if (n < 2) return w;
@@ -684,7 +695,8 @@ int launch(const char *op, const PackedArgs &a, hipStream_t st) {
                      a);
   if (a.n_pieces > 1)
     hipLaunchKernelGGL((q8_prefill_reduce_kernel<T, HD>),
-                       dim3(a.n_tiles * a.n_kv, 4), dim3(256), 0, st, a);
+                       dim3(a.n_tiles * a.n_kv, kRows * HD / 1024), dim3(256), 0,
+                       st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
 }
@@ -705,8 +717,9 @@ size_t rvkv_q8_prefill_workspace_bytes(const rvkv_q8_pool *pool,
                                        uint32_t n_heads, uint32_t max_blocks,
                                        int32_t window) {
   if (!pool || n_heads == 0 || n_heads % pool->n_kv) return 0;
+  // (f16 is cut into as many pieces as f32, or more)
   return layout(pool, total_rows, batch, n_heads, max_blocks,
-                window > 0 ? (uint32_t)window : 0).bytes;
+                window > 0 ? (uint32_t)window : 0, RVKV_F16).bytes;
 }
 
 int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
@@ -738,7 +751,7 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
     return fail(RVKV_EINVAL, op, "q and out must be 16-byte aligned");
   const uint32_t bsg = pool->block_size / 16;
   const uint32_t win = window > 0 ? (uint32_t)window : 0;
-  Layout w = layout(pool, total_rows, batch, n_heads, max_blocks, win);
+  Layout w = layout(pool, total_rows, batch, n_heads, max_blocks, win, dtype);
   if (!ws) w.n_pieces = 1;
   if (w.n_pieces > 1 && ws_bytes < w.bytes)
     return fail(RVKV_EINVAL, op, "workspace smaller than the required bytes");

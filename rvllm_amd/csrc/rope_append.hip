@@ -9,8 +9,12 @@
 // An 8-bit row takes scale = f32(max |x| / 127) and code = rint(x / scale),
 // ties to even. f64 keeps the angles of positions near 2^32 to 1e-7 and the
 // codes equal to the definition's: values next to a code's border would
-// round to either side of it in f32 (VALU f64 runs at the f32 rate here, and
-// the launch is bound by HBM).
+// round to either side of it in f32.
+//
+// 8191 packed rows of 16 + 8 heads of 128, normed, f16, into 8-bit cells: 65 us
+// for 118 MB (HBM moves those bytes and no more); 8000 rows of 32 + 8 heads of
+// 64 without norms 34 us for 91 MB. Bound by its waves' waits, half of their
+// cycles, at three waves a SIMD, and the f64 arithmetic of K beside them.
 #include <type_traits>
 
 #include "q8.h"
@@ -505,6 +509,15 @@ int rope_append(const char *op, int cell, int device, hipStream_t st,
   if ((uintptr_t)a.q % eb || (uintptr_t)a.k % eb || (uintptr_t)a.v % eb ||
       (uintptr_t)a.q_out % eb)
     return fail(RVKV_EINVAL, op, "q/k/v/q_out must be aligned to their type");
+  // (a head's partners are read while others are written)
+  const auto apart = [&](const void *in, uint64_t stride, uint64_t width) {
+    const uintptr_t x = (uintptr_t)in, y = (uintptr_t)a.q_out;
+    return !in || !y || x + ((a.rows - 1) * stride + width) * eb <= y ||
+           y + (uint64_t)a.rows * a.n_heads * a.hd * eb <= x;
+  };
+  if (!apart(a.q, a.q_stride, (uint64_t)a.n_heads * a.hd) ||
+      !apart(a.k, a.k_stride, kv_row) || !apart(a.v, a.v_stride, kv_row))
+    return fail(RVKV_EINVAL, op, "q_out overlaps q, k or v");
   const int rc = rvkv_detail::q8_device(op, device);
   if (rc) return rc;
   a.interleaved = interleaved;

@@ -181,8 +181,14 @@ class HipQ8Storage:
 
     def _scratch(self, op, ws, need):
         if ws is None:
-            return (torch.empty(need, dtype=torch.uint8, device=self.device)
-                    if need else None)
+            if not need:
+                return None
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            # (the pool's stream may be another than torch's: the memory is
+            # not handed out again before the work there is done)
+            if torch.cuda.current_stream(self.device) != self.stream:
+                ws.record_stream(self.stream)
+            return ws
         if ws.device != self.device or not ws.is_contiguous():
             raise RvkvError(f"{op}: workspace must be contiguous and on the "
                             "storage's device")

@@ -197,6 +197,15 @@ def test_q8_append_runs_of_slots(first):
         assert (st.scales(0, which) != 0).sum() == (rows - 1) * kv
 
 
+def test_q8_pool_refuses_host_memory():
+    from rvllm_amd._lib import RvkvError
+    for pin in (False, True):
+        mem = torch.zeros(1 << 16, dtype=torch.uint8, pin_memory=pin)
+        at = -mem.data_ptr() % 256
+        with pytest.raises(RvkvError, match="not the current device's"):
+            HipQ8Storage(1, 2, 16, 1, 64, memory=mem[at:])
+
+
 # -- decode -------------------------------------------------------------------
 
 def filled(nb, bs, kv, hd, seed, layers=1):

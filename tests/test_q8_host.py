@@ -112,6 +112,8 @@ def test_append_refuses():
                                      pos, inv.data_ptr(), rot, inter, f, n, n,
                                      q.data_ptr())
 
+    assert raw(rows=1) == _lib.RVKV_EINVAL  # (q_out is q)
+    assert b"overlaps" in L.rvkv_last_error()
     assert raw(qs=255) == _lib.RVKV_EINVAL
     assert raw(ks=127) == _lib.RVKV_EINVAL
     assert raw(dtype=5) == _lib.RVKV_EINVAL
