@@ -11,10 +11,12 @@
 // codes equal to the definition's: values next to a code's border would
 // round to either side of it in f32.
 //
-// 8191 packed rows of 16 + 8 heads of 128, normed, f16, into 8-bit cells: 65 us
-// for 118 MB (HBM moves those bytes and no more); 8000 rows of 32 + 8 heads of
-// 64 without norms 34 us for 91 MB. Bound by its waves' waits, half of their
-// cycles, at three waves a SIMD, and the f64 arithmetic of K beside them.
+// 8191 packed rows of 16 + 8 heads of 128, normed, f16, into 8-bit cells: 64 us
+// for 118 MB; 8000 rows of 32 + 8 heads of 64 without norms 34 us for 91 MB.
+// The vector units are busy 55 % of the time, f64 of K and the codes' borders
+// first, and the waves, four a SIMD, wait half of theirs. V codes of a block
+// are written by four workgroups on four XCDs, 83 MB where 51 are needed;
+// neighbouring tokens on one XCD write 50 and take 69 us.
 #include <type_traits>
 
 #include "q8.h"
