@@ -126,9 +126,10 @@ __global__ void __launch_bounds__(256)
 // more than a rounded one. Larger groups take n_sub workgroups.
 //
 // A wave takes 64 keys at a time; a workgroup's four waves take turns, or a
-// wave has a partition of its own (see cut). Row 4g + i of S tile t is key 16g + 4t + i, so lane group g of the result
-// holds keys 16g .. 16g+15: the order in which the V' P product takes its
-// weights from the same registers, and 16 keys of one dim are 16 bytes of a
+// wave has a partition of its own (see cut). Row 4g + i of S tile t is key
+// 16g + 4t + i, so lane group g of the result holds keys 16g .. 16g+15: the
+// order in which the V' P product takes its weights from the same registers,
+// and 16 keys of one dim are 16 bytes of a
 // V record. No operand passes through LDS, only the scales do.
 //
 // Bound by the reads of the cache at two waves a SIMD (199 registers at hd 128;
@@ -392,7 +393,8 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2)
       }
       if (more) load_k(pk1);
       if (masked) {
-        __builtin_amdgcn_sched_barrier(0);  // (a branch, no selects on every tile)
+        // (a branch, no selects on every tile)
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = keep >> j & 1 ? s[j] : kNone;
       }

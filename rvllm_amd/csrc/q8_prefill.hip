@@ -26,6 +26,8 @@
 // GFLOP in 284 us, 660 TFLOP/s; 4 prompts up to 4000 at 32 + 8 heads of 64: 555.
 // With 64 rows a wave, each LDS operand feeding two products, the accumulators
 // move between the register files every tile: 514 us.
+#include <atomic>
+
 #include "q8.h"
 
 using rvkv_detail::fail;
@@ -81,17 +83,27 @@ struct Work {
   uint64_t pos0, read;                     //  below 2^32)
 };
 
-// Sum and maximum over a wave.
+// Sum and maximum over a wave, by DPP and swaps of rows (by LDS exchanges each
+// took ~500 cycles, and a workgroup's search for its tile takes ten).
+template <typename F>
+__device__ __forceinline__ uint32_t over_wave(uint32_t x, F f) {
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return uniform(f((uint32_t)b[0], (uint32_t)b[1]));
+}
 __device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += (uint32_t)__shfl_xor((int)x, o);
-  return uniform(x);
+  return over_wave(x, [](uint32_t u, uint32_t v) { return u + v; });
 }
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1)
-    x = max(x, (uint32_t)__shfl_xor((int)x, o));
-  return uniform(x);
+  return over_wave(x, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t x) {
+  return over_wave(x, [](uint32_t u, uint32_t v) { return u < v ? u : v; });
 }
 
 // The t-th tile of the launch; false: there are no more than t. Every wave
@@ -262,17 +274,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     any_hi = max(any_hi, key_hi);
   }
   // Keys that every row of this wave sees, and that any does.
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, o));
-    all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, o));
-    any_hi = max(any_hi, (uint32_t)__shfl_xor((int)any_hi, o));
-    any_lo = min(any_lo, (uint32_t)__shfl_xor((int)any_lo, o));
-  }
-  all_lo = uniform(all_lo);
-  all_hi = uniform(all_hi);
-  any_lo = uniform(any_lo);
-  any_hi = uniform(any_hi);
+  all_lo = wave_max(all_lo);
+  all_hi = wave_min(all_hi);
+  any_lo = wave_min(any_lo);
+  any_hi = wave_max(any_hi);
 
   const uint32_t *table = a.tables + (size_t)w.seq * a.max_blocks;
   const uint32_t last_granule = w.end ? (w.end - 1) / 16 : 0;
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   const auto put = [&](Tile<HD> &s) {
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
-      half8v *k = reinterpret_cast<half8v *>(&s.k[k_key + kStep * i][k_ch * 16]);
+      half8v *k =
+          reinterpret_cast<half8v *>(&s.k[k_key + kStep * i][k_ch * 16]);
       k[0] = codes_to_half8(kraw[i].x, kraw[i].y);
       k[1] = codes_to_half8(kraw[i].z, kraw[i].w);
     }
@@ -453,7 +459,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
         for (int i = 0; i < 4; ++i) sc[kh][r + i] *= k4[i];
       }
     if (masked) {  // (uniform over the wave)
-      __builtin_amdgcn_sched_barrier(0);  // (a branch, no selects on every tile)
+      // (a branch, no selects on every tile)
+      __builtin_amdgcn_sched_barrier(0);
       const uint32_t from = kt + 8 * h - key_lo;
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
@@ -653,7 +660,7 @@ struct Layout {
 // far as the host can tell them from the width of the table and the window, in
 // pieces of at least 128. 450 rows behind 7700 keys, 32 + 8 heads of 64: f32
 // 109 us for 512 workgroups, 164 for 256, 137 for 768; f16 74 us for 768, 83
-// for 512, 136 for 256.
+// for 512, 136 for 256 (before the waves' search for their tile was shortened).
 Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
               uint32_t n_heads, uint32_t max_blocks, uint32_t window,
               rvkv_dtype dtype) {
@@ -684,28 +691,34 @@ Layout layout(const rvkv_q8_pool *p, uint32_t total_rows, uint32_t batch,
 }
 
 template <typename T, int HD, bool SPLIT>
-int launch(const char *op, const PackedArgs &a, hipStream_t st) {
+int launch(const char *op, const PackedArgs &a, int device, hipStream_t st) {
   const size_t lds = 2 * sizeof(Tile<HD>);
-  static const hipError_t set = hipFuncSetAttribute(
-      reinterpret_cast<const void *>(&q8_prefill_kernel<T, HD, SPLIT>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  if (set != hipSuccess) return hip_fail(op, set);
+  // (once on every device: bit d of done)
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(done.load() & bit)) {
+    const hipError_t e = hipFuncSetAttribute(
+        reinterpret_cast<const void *>(&q8_prefill_kernel<T, HD, SPLIT>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return hip_fail(op, e);
+    done.fetch_or(bit);
+  }
   hipLaunchKernelGGL((q8_prefill_kernel<T, HD, SPLIT>),
                      dim3(a.n_tiles * a.n_kv * a.n_pieces), dim3(256), lds, st,
                      a);
   if (a.n_pieces > 1)
     hipLaunchKernelGGL((q8_prefill_reduce_kernel<T, HD>),
-                       dim3(a.n_tiles * a.n_kv, kRows * HD / 1024), dim3(256), 0,
-                       st, a);
+                       dim3(a.n_tiles * a.n_kv, kRows * HD / 1024), dim3(256),
+                       0, st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? RVKV_OK : hip_fail(op, e);
 }
 
 template <typename T, bool SPLIT>
-int launch(const char *op, const PackedArgs &a, hipStream_t st) {
-  if (a.hd <= 64) return launch<T, 64, SPLIT>(op, a, st);
-  if (a.hd <= 128) return launch<T, 128, SPLIT>(op, a, st);
-  return launch<T, 256, SPLIT>(op, a, st);
+int launch(const char *op, const PackedArgs &a, int device, hipStream_t st) {
+  if (a.hd <= 64) return launch<T, 64, SPLIT>(op, a, device, st);
+  if (a.hd <= 128) return launch<T, 128, SPLIT>(op, a, device, st);
+  return launch<T, 256, SPLIT>(op, a, device, st);
 }
 
 }  // namespace
@@ -789,8 +802,9 @@ int rvkv_q8_packed_prefill(const rvkv_q8_pool *pool, uint32_t layer,
   a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.ml_off);
   a.bsg_log2 = bsg & (bsg - 1) ? -1 : __builtin_ctz(bsg);
   a.qscale = scale * kLog2e;
-  return dtype == RVKV_F16 ? launch<_Float16, false>(op, a, pool->stream)
-                           : launch<float, true>(op, a, pool->stream);
+  return dtype == RVKV_F16
+             ? launch<_Float16, false>(op, a, pool->device, pool->stream)
+             : launch<float, true>(op, a, pool->device, pool->stream);
 }
 
 }  // extern "C"
