@@ -148,6 +148,7 @@ class HipQ8Storage:
               "ctx_len * head_dim")
         _need(out_k.dtype == out_v.dtype and out_k.dtype in _DT,
               "kv_gather: outputs must both be float32 or float16")
+        _on(self, "kv_gather", (plan.block_idx, out_k, out_v))
         check(self._L.rvkv_q8_gather(
             self._pool, layer, _ptr(plan.block_idx), plan.batch,
             plan.max_blocks, plan.ctx_len, _ptr(out_k), _ptr(out_v),
@@ -157,6 +158,10 @@ class HipQ8Storage:
         """Copies src[i] -> dst[i] for all layers, K and V."""
         _need(src.numel() == dst.numel(),
               "copy_blocks: src and dst have different lengths")
+        for t in (src, dst):
+            _need(t.dtype == torch.int32 and t.is_contiguous(),
+                  "copy_blocks: src and dst must be contiguous int32")
+        _on(self, "copy_blocks", (src, dst))
         check(self._L.rvkv_q8_copy_blocks(self._pool, _ptr(src), _ptr(dst),
                                           src.numel()))
 

@@ -182,6 +182,29 @@ def test_prefill_refuses():
     assert empty.shape == (0, 4, 64)
 
 
+def test_gather_and_copy_refuse():
+    from rvllm_amd.kv_storage import HipGatherPlan
+    st = host_pool()
+    plan = HipGatherPlan([([0, 1], 20)], device="cpu")
+    out = torch.zeros(1, 2, 20, 64)
+    for match, k, v in [("output length", out[:, :, :19], out),
+                        ("output length", out.transpose(1, 2), out),
+                        ("float32 or float16", out, out.half()),
+                        ("float32 or float16", out.double(), out.double())]:
+        with pytest.raises(RvkvError, match=match):
+            st.gather(0, plan, k, v)
+    with pytest.raises(RvkvError, match="layer"):
+        st.gather(9, plan, out, out)
+    with pytest.raises(RvkvError, match="max_blocks \\* block_size"):
+        st.gather(0, HipGatherPlan([([0], 20)], device="cpu"), out, out)
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RvkvError, match="different lengths"):
+        st.copy_blocks(i, i[:2])
+    with pytest.raises(RvkvError, match="contiguous int32"):
+        st.copy_blocks(i.long(), i.long())
+    st.copy_blocks(i[:0], i[:0])  # nothing to do
+
+
 def test_a_call_without_a_device_fails_and_says_so():
     if torch.cuda.is_available():
         pytest.skip("needs a host without a GPU")
